@@ -7,12 +7,14 @@ nothing once its workspace exists) and launch on torch's current stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import library
+from .packed import GROUPS, FewRowsPlan, PackedWeights, few_rows_plan
 from ..csrc import build
 
 F32, BF16 = 0, 1
@@ -177,6 +179,7 @@ class CudaKernels:
         self._attention_tc_libs = {}
         self._attention_tied_libs = {}
         self.use_tcgen05_attention = True
+        self._packed_plans: Dict[tuple, FewRowsPlan] = {}
         self._partial_bufs = [None, None]
         self._partial_turn = 0
         self._partial_stamps = [0, 0]     # how often each of the two arrays has been handed out
@@ -465,6 +468,7 @@ class CudaKernels:
                     32: "a wait that ran out (experts' product: tensor-core issuer)",
                     33: "a wait that ran out (experts' product: epilogue)",
                     34: "a wait that ran out (experts' product: accumulator hand-over)",
+                    41: "a wait that ran out (product with a matrix in 4 bits: few rows)",
                     **{c: f"a wait that ran out (tcgen05 attention, point {c})" for c in range(21, 30)}}.get(code, f"code {code}")
             raise KernelError(f"a kernel refused {what}")
 
@@ -513,8 +517,8 @@ class CudaKernels:
         sums for a fused consumer; None if this product is not one that is split
         (then use ``linear``).  ``max_splits``: at most so many splits (a consumer
         that fetches only so many partial sums in one go says so)."""
-        if isinstance(x, ScaledRows):
-            return None                  # many rows: such a product is not split
+        if isinstance(x, ScaledRows) or isinstance(w, PackedWeights):
+            return None                  # many rows, or a matrix in 4 bits: such a product is not split
         if not (self.use_tensor_cores and self.fuse_split_products and x.is_cuda
                 and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16):
             return None
@@ -590,7 +594,13 @@ class CudaKernels:
     def linear_swiglu(self, x: torch.Tensor, w_interleaved: torch.Tensor, out: torch.Tensor, kind: str = "silu") -> bool:
         """out[M, I] = act(x @ gate^T) * (x @ up^T) in one kernel (``kind``: "silu" or "gelu_tanh"), with the weights
         as ``interleave_gate_up`` arranges them.  False if the kernel refuses the
-        shapes (the caller then takes the two-kernel way)."""
+        shapes (the caller then takes the two-kernel way).  ``w_interleaved`` may be a pair of matrices in 4 bits
+        (``pack_gate_up``): any x and out of the two types, never False."""
+        if isinstance(w_interleaved, PackedWeights):
+            if kind not in self._GATED_EPILOGUES:
+                raise KernelError(f"linear_swiglu: one of {sorted(self._GATED_EPILOGUES)}")
+            self._packed_product(x, w_interleaved, out, None, kind, "linear_swiglu")
+            return True
         epilogue = self._GATED_EPILOGUES[kind][0]
         if isinstance(x, ScaledRows):
             if self._linear_of_scaled(x, w_interleaved, out, swiglu=epilogue):
@@ -704,7 +714,10 @@ class CudaKernels:
         bfloat16 products read w before the kernel ahead of them has ended: it is constant, or no kernel of this package
         in flight on the stream writes it (32-bit products wait first).
         With ``defer`` (together with a residual that aliases out, or without one) a split
-        product is left pending -- the caller adds it, or takes it for ``out`` -- and is returned."""
+        product is left pending -- the caller adds it, or takes it for ``out`` -- and is returned.
+        ``w`` may be PackedWeights (not a pair): any x and out of the two types."""
+        if isinstance(w, PackedWeights):
+            return self._packed_product(x, w, out, residual, None, "linear")
         if isinstance(x, ScaledRows):
             if residual is None and self._linear_of_scaled(x, w, out, swiglu=False):
                 return None
@@ -760,6 +773,139 @@ class CudaKernels:
             _ptr(x), _code(x), _ptr(w), _code(w), _ptr(out), _code(out), _ptr(residual), M, N, K,
             x.stride(0), w.stride(0), out.stride(0),
             residual.stride(0) if residual is not None else 0, self._stream()), "linear")
+
+    # ---- matrices in 4 bits
+    def pack_weights(self, w: torch.Tensor, group: int = 64) -> PackedWeights:
+        """w [rows, columns] in 4 bits: groups of ``group`` (32, 64 or 128) neighbouring columns share a scale, the element
+        of largest magnitude (the first of equals) over -8, rounded to bfloat16; an element is the nearest multiple
+        (ties to the even one) of -8 ... 7 scales.  A group with an infinity or NaN becomes NaN.  Allocates."""
+        return self._pack(w, None, group, "pack_weights")
+
+    def pack_gate_up(self, gate: torch.Tensor, up: torch.Tensor, group: int = 64) -> PackedWeights:
+        """A pair of matrices of one shape in 4 bits, for ``linear_swiglu``."""
+        if gate.shape != up.shape or gate.dtype != up.dtype:
+            raise KernelError(f"pack_gate_up: gate {tuple(gate.shape)} {gate.dtype} and up {tuple(up.shape)} {up.dtype}")
+        return self._pack(gate, up, group, "pack_gate_up")
+
+    def _pack(self, w: torch.Tensor, up: Optional[torch.Tensor], group: int, what: str) -> PackedWeights:
+        self._packed_sizes(w, group, what)
+        for t in (w, up):
+            if t is not None:
+                _rows_contiguous(t, what)
+        out = self._packed_room(w.shape[0], w.shape[1], group, up is not None)
+        code = _code(w)
+        with self._current_device():
+            self.launches += 1
+            _check(self.lib.chibi_pack_weights(_ptr(w), _ptr(up), code, w.shape[0], w.shape[1], w.stride(0),
+                                               up.stride(0) if up is not None else 0, group, _ptr(out.data), self._stream()), what)
+        return out
+
+    def pack_codes(self, codes: torch.Tensor, scales: torch.Tensor, group: int, up_codes: Optional[torch.Tensor] = None,
+                   up_scales: Optional[torch.Tensor] = None) -> PackedWeights:
+        """A matrix (or, with ``up_codes`` and ``up_scales``, a pair) whose whole numbers (int8 [rows, columns], -8 ... 7)
+        and scales (bfloat16 [rows, groups of a row]) are known.  Allocates, and reads the codes' range on the host."""
+        if (up_codes is None) != (up_scales is None):
+            raise KernelError("pack_codes: up_codes and up_scales come together")
+        self._packed_sizes(codes, group, "pack_codes")
+        for q, s in ((codes, scales), (up_codes, up_scales)):
+            if q is None:
+                continue
+            self._on_this_device("pack_codes", q, s)
+            _rows_contiguous(q, "pack_codes: codes")
+            _rows_contiguous(s, "pack_codes: scales")
+            if q.dtype != torch.int8 or q.shape != codes.shape:
+                raise KernelError("pack_codes: codes are int8, a pair's of one shape")
+            if s.dtype != torch.bfloat16 or s.shape != (q.shape[0], -(-q.shape[1] // group)):
+                raise KernelError(f"pack_codes: scales must be bfloat16 [rows, groups], got {s.dtype} {tuple(s.shape)}")
+            if int(q.min()) < -8 or int(q.max()) > 7:
+                raise KernelError("pack_codes: codes outside -8 ... 7")
+        out = self._packed_room(codes.shape[0], codes.shape[1], group, up_codes is not None)
+        with self._current_device():
+            self.launches += 1
+            _check(self.lib.chibi_pack_codes(_ptr(codes), _ptr(scales), _ptr(up_codes), _ptr(up_scales), codes.shape[0], codes.shape[1],
+                                             codes.stride(0), scales.stride(0), up_codes.stride(0) if up_codes is not None else 0,
+                                             up_scales.stride(0) if up_scales is not None else 0, group, _ptr(out.data),
+                                             self._stream()), "pack_codes")
+        return out
+
+    def unpack_weights(self, w: PackedWeights, out: torch.Tensor) -> None:
+        """The values of a matrix in 4 bits, rounded to out's type; of a pair, gate's rows before up's."""
+        self._on_this_device("unpack_weights", w.data, out)
+        _rows_contiguous(out, "unpack_weights: out")
+        if out.shape != w.shape:
+            raise KernelError(f"unpack_weights: out {tuple(out.shape)}, the matrix is {tuple(w.shape)}")
+        code = _code(out)
+        with self._current_device():
+            self.launches += 1
+            _check(self.lib.chibi_unpack_weights(_ptr(w.data), w.rows, w.columns, int(w.paired), w.group, _ptr(out), code,
+                                                 out.stride(0), self._stream()), "unpack_weights")
+
+    def _current_device(self):
+        """A context in which launches go to these kernels' device (nothing to do where it is the current one)."""
+        if torch.cuda.current_device() == self._device_index:
+            return contextlib.nullcontext()
+        return torch.cuda.device(self._device_index)
+
+    def _on_this_device(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
+        _need_cuda(*tensors)
+        for t in tensors:
+            if t is not None and t.device.index != self._device_index:
+                raise KernelError(f"{what}: a tensor on {t.device}, these kernels run on cuda:{self._device_index}")
+
+    def _packed_sizes(self, w: torch.Tensor, group: int, what: str) -> None:
+        if group not in GROUPS:
+            raise KernelError(f"{what}: groups of {group} columns (one of {GROUPS})")
+        if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
+            raise KernelError(f"{what}: a matrix of {tuple(w.shape)}")
+        self._on_this_device(what, w)
+
+    def _packed_room(self, rows: int, columns: int, group: int, paired: bool) -> PackedWeights:
+        data = torch.empty(PackedWeights.bytes_for(rows, columns, group, paired), dtype=torch.uint8, device=self.device)
+        return PackedWeights(data, rows, columns, group, paired)
+
+    def packed_plan(self, w: PackedWeights, m: int, x32: bool) -> FewRowsPlan:
+        """How the product of m rows of x with this matrix is shared out (kernels/packed.py)."""
+        key = (w.rows, w.columns, w.paired, w.group, m, x32)
+        plan = self._packed_plans.get(key)
+        if plan is None:
+            lib, x = self.lib, int(x32)
+            plan = few_rows_plan(w.rows, w.columns, w.paired, m,
+                                 lambda tokens, splits, batch, depth: lib.chibi_packed_few_rows_kb(x, w.group, w.columns, tokens, splits, batch, depth),
+                                 lambda tokens, splits, kb: lib.chibi_packed_few_rows_clusters(x, w.group, tokens, splits, kb))
+            if plan is None:
+                raise KernelError(f"a product over {w.columns} columns in 4 bits: more than the kernel holds")
+            if len(self._packed_plans) > 4096:
+                self._packed_plans.clear()
+            self._packed_plans[key] = plan
+        return plan
+
+    def _packed_product(self, x, w: PackedWeights, out: torch.Tensor, residual: Optional[torch.Tensor], kind: Optional[str],
+                        what: str) -> None:
+        if isinstance(x, ScaledRows):
+            x = x.materialise()
+        if w.paired != (kind is not None):
+            raise KernelError(f"{what}: a pair of matrices (pack_gate_up) belongs to linear_swiglu, any other to linear")
+        self._on_this_device(what, x, w.data, out, residual)
+        _rows_contiguous(x, f"{what}: x")
+        _rows_contiguous(out, f"{what}: out")
+        M, K = x.shape
+        if K != w.columns or out.shape != (M, w.rows):
+            raise KernelError(f"{what}: shapes x {tuple(x.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
+        if residual is not None:
+            _rows_contiguous(residual, f"{what}: residual")
+            if residual.dtype != torch.float32 or residual.shape != out.shape:
+                raise KernelError(f"{what}: residual must be float32 [M, N]")
+        x_code, out_code = _code(x), _code(out)
+        if M == 0:
+            return
+        with self._current_device():
+            plan = self.packed_plan(w, M, x_code == F32)
+            self.launches += 1
+            self.tensor_core_calls += 1
+            _check(self.lib.chibi_packed_few_rows(
+                _ptr(w.data), w.group, w.rows, w.columns, int(w.paired), _ptr(x), x_code, x.stride(0), M, _ptr(out), out_code, out.stride(0),
+                _ptr(residual), residual.stride(0) if residual is not None else 0, self.ACTIVATIONS[kind] if kind else 0,
+                plan.splits, plan.along_k, plan.batch, plan.depth, plan.tokens, plan.clusters, _ptr(self.error), self._stream()), what)
 
     def qk_norm_rope_append(self, qkv: torch.Tensor, q_out: torch.Tensor,
                             k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
