@@ -1,0 +1,458 @@
+// The product of many bfloat16 rows of x with a matrix held in 4 bits (packed.cuh), on tcgen05.
+//
+//   out[m][n] = sum over groups of s[n][g] * (sum over the group of q[n][k] x[m][k])
+//
+// The matrix's 128 rows of a tile are the instruction's rows, TOKENS rows of x its columns.  Warps that do nothing else turn
+// codes into bfloat16 whole numbers (exact) and write them to TMEM, where they are the A operand: shared memory carries only
+// the rows of x and the codes themselves.  Each group's sum is an accumulator of its own in TMEM; two warpgroups read it, each
+// half of the columns, and add it times the row's scale to sums in registers.  So nothing is rounded but 32-bit sums, and a
+// lane's row has one scale for all of its columns.  A thread's sums are an output column of 32 lanes: stores are whole
+// lines without a detour.
+//
+// What bounds it: with 128 tokens a tile, a block of 128 columns takes the tensor cores 512 cycles (8,192 multiply-adds
+// a cycle and SM for 128 x 128 x 128), the four converting warps some 250 instructions each, the eight adding warps 64 columns for each
+// group; at groups of 32 reading TMEM (four times as often as at 128) takes as long as the products.
+//
+// Few tiles: `splits` CTAs of a cluster share a tile's columns; their sums go to shared memory and each CTA adds up a
+// share of them, CTA by CTA in one order.
+#define CHIBI_UNIT packed_tcgen05
+#define CHIBI_UNIT_ID 20
+#include "packed.cuh"
+#include "sm100.cuh"
+#include "split_f32.cuh"
+#include "tensor_map.cuh"
+
+namespace chibi {
+namespace {
+
+constexpr int PT_THREADS = 512;                  // loader, issuer, 2 idle warps | 4 converting | 8 adding
+constexpr int PT_ROWS = 128;
+constexpr int PT_SCALE_SLOTS = 8;                // blocks of columns whose scales are kept
+
+template <int TOKENS, int GROUP_BLOCKS> struct PackedTile {
+    static constexpr int GROUPS = 4 / GROUP_BLOCKS;
+    static constexpr int RECORD = PACKED_CODE_BYTES + GROUPS * 64;
+    static constexpr int X_BYTES = TOKENS * PACKED_COLS * 2, CODE_BYTES = PT_ROWS / PACKED_ROWS * RECORD;
+    static constexpr int CODE_ROOM = (CODE_BYTES + 1023) / 1024 * 1024;
+    static constexpr int STAGE = X_BYTES + CODE_ROOM;
+    static constexpr int SCALES = PT_SCALE_SLOTS * GROUPS * PT_ROWS * 4;
+    static constexpr int BUDGET = 226 * 1024 - 1024 - SCALES - 1024;
+    static constexpr int STAGES = BUDGET / STAGE > 6 ? 6 : BUDGET / STAGE;
+    // accumulators (one for each group on its way) and operand blocks in TMEM's 512 columns
+    static constexpr int SUMS = TOKENS <= 64 ? 4 : 2, OPERANDS = (512 - SUMS * TOKENS) / 64 > 4 ? 4 : (512 - SUMS * TOKENS) / 64;
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + SCALES + (2 * STAGES + 2 * OPERANDS + 2 * SUMS) * 8 + 16;
+    static_assert(STAGES >= 2 && OPERANDS >= 2, "");
+    // Block i's scales go where block i - 8's were.  Its operand's place is free when the products of block i - OPERANDS are
+    // done, which began when all groups but the last SUMS up to there had been added up: those of block i - 8 among them.
+    static_assert(SUMS <= (PT_SCALE_SLOTS - OPERANDS) * GROUPS, "");
+    static_assert(STAGES * STAGE >= TOKENS * PT_ROWS * 4, "a tile's sums fit where the stages were");
+};
+
+struct PackedProduct {
+    const uint8_t* data;
+    int row_blocks, chunks;                      // blocks of 32 rows, of 128 columns
+    int n, pair;
+    int m;
+    void* out;
+    int out_type;
+    long long out_stride;
+    const float* residual;
+    long long residual_stride;
+    int act;                                     // pairs: 1 gelu with tanh, 2 silu
+    int splits, tiles, token_tiles;
+    int* error;
+};
+
+__device__ __forceinline__ void peer_shared_f32x4(uint32_t own_smem_addr, uint32_t rank, float (&v)[4])
+{
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                 : "r"(sm100::peer_smem_addr(own_smem_addr, rank))
+                 : "memory");
+}
+
+__device__ __forceinline__ void packed_write(const PackedProduct& p, long long m, int at, float v)
+{
+    if (p.out_type == CHIBI_F32)
+        static_cast<float*>(p.out)[m * p.out_stride + at] = v;
+    else
+        static_cast<__nv_bfloat16*>(p.out)[m * p.out_stride + at] = from_f32<__nv_bfloat16>(v);
+}
+
+template <int TOKENS, int GROUP_BLOCKS>
+__global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const __grid_constant__ CUtensorMap map_x, const PackedProduct p)
+{
+    using namespace sm100;
+    using T = PackedTile<TOKENS, GROUP_BLOCKS>;
+    constexpr int GROUPS = T::GROUPS, RECORD = T::RECORD, STAGES = T::STAGES, OPERANDS = T::OPERANDS, SUMS = T::SUMS;
+    constexpr int COLS = TOKENS / 2;             // of an adding warpgroup
+    pdl_trigger();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* scales = reinterpret_cast<float*>(smem + STAGES * T::STAGE);          // [slot][group][row]
+    uint64_t* full = reinterpret_cast<uint64_t*>(scales + T::SCALES / 4);         // a stage's codes and rows of x are there
+    uint64_t* empty = full + STAGES;
+    uint64_t* operand_full = empty + STAGES;
+    uint64_t* operand_empty = operand_full + OPERANDS;
+    uint64_t* sums_full = operand_empty + OPERANDS;
+    uint64_t* sums_empty = sums_full + SUMS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_empty + SUMS);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = p.splits > 1 ? (int)cluster_cta_rank() : 0;
+    const int c0 = (int)((long long)p.chunks * rank / p.splits), c1 = (int)((long long)p.chunks * (rank + 1) / p.splits);
+    const int first_tile = blockIdx.x / p.splits, tile_step = gridDim.x / p.splits;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1 + 4);         // the products have read x, the converting warps the codes
+        }
+        for (int s = 0; s < OPERANDS; ++s) {
+            mbar_init(&operand_full[s], 4);
+            mbar_init(&operand_empty[s], 1);
+        }
+        for (int s = 0; s < SUMS; ++s) {
+            mbar_init(&sums_full[s], 1);
+            mbar_init(&sums_empty[s], 8);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem_sums = *tmem_slot, tmem_operands = tmem_sums + SUMS * TOKENS;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            tma_prefetch_descriptor(&map_x);
+            const int per_tile = c1 - c0;
+            const long long total = first_tile < p.tiles ? (long long)((p.tiles - 1 - first_tile) / tile_step + 1) * per_tile : 0;
+            // the codes are constant: those of the first stages are asked for before the kernel ahead has ended
+            auto load_codes = [&](long long i) {
+                const int tile = first_tile + (int)(i / per_tile) * tile_step, chunk = c0 + (int)(i % per_tile);
+                const int s = (int)(i % STAGES), rb = tile / p.token_tiles * (PT_ROWS / PACKED_ROWS);
+                const int records = min(PT_ROWS / PACKED_ROWS, p.row_blocks - rb);
+                mbar_arrive_expect_tx(&full[s], T::X_BYTES + records * RECORD);
+                for (int j = 0; j < records; ++j)
+                    bulk_load(smem + s * T::STAGE + T::X_BYTES + j * RECORD, p.data + ((long long)(rb + j) * p.chunks + chunk) * RECORD,
+                              RECORD, &full[s]);
+            };
+            auto load_x = [&](long long i) {
+                const int tile = first_tile + (int)(i / per_tile) * tile_step, chunk = c0 + (int)(i % per_tile);
+                const int s = (int)(i % STAGES), token0 = tile % p.token_tiles * TOKENS;
+                uint8_t* dst = smem + s * T::STAGE;
+                tma_load_2d(dst, &map_x, &full[s], chunk * PACKED_COLS, token0);
+                tma_load_2d(dst + T::X_BYTES / 2, &map_x, &full[s], chunk * PACKED_COLS + 64, token0);
+            };
+            const int early = total < STAGES ? (int)total : STAGES;
+            for (int i = 0; i < early; ++i)
+                load_codes(i);
+            pdl_wait();
+            for (int i = 0; i < early; ++i)
+                load_x(i);
+            long long i = early;
+            for (; i < total; ++i) {
+                if (!mbar_wait(&empty[i % STAGES], (uint32_t)(i / STAGES - 1) & 1, p.error, 42))
+                    break;
+                load_codes(i);
+                load_x(i);
+            }
+            // every copy has landed before this CTA's shared memory is anybody else's
+            for (long long j = i > STAGES ? i - STAGES : 0; j < i; ++j)
+                mbar_wait(&full[j % STAGES], (uint32_t)(j / STAGES) & 1, p.error, 42);
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            constexpr uint32_t idesc = make_idesc_bf16_f32(PT_ROWS, TOKENS);
+            constexpr int STEPS = GROUP_BLOCKS * 2;          // 16-column steps of a group
+            uint32_t i = 0, a = 0;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step)
+                for (int chunk = c0; ok && chunk < c1; ++chunk, ++i) {
+                    const uint32_t s = i % STAGES, o = i % OPERANDS;
+                    if (!mbar_wait(&full[s], (i / STAGES) & 1, p.error, 43) || !mbar_wait(&operand_full[o], (i / OPERANDS) & 1, p.error, 43)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t x_addr = smem_addr(smem + s * T::STAGE);
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g, ++a) {
+                        const uint32_t d = a % SUMS;
+                        if (a >= SUMS && !mbar_wait(&sums_empty[d], (a / SUMS - 1) & 1, p.error, 44)) {
+                            ok = false;
+                            break;
+                        }
+                        tcgen05_fence_after();
+#pragma unroll
+                        for (int k = 0; k < STEPS; ++k) {
+                            const int step = g * STEPS + k;
+                            tcgen05_mma_bf16_a_tmem(tmem_sums + d * TOKENS, tmem_operands + o * 64 + step * 8,
+                                                    make_kmajor_sw128_desc(x_addr + (step >> 2) * (T::X_BYTES / 2) + (step & 3) * 32), idesc,
+                                                    k > 0 ? 1u : 0u);
+                        }
+                        tcgen05_commit(&sums_full[d]);
+                    }
+                    tcgen05_commit(&operand_empty[o]);
+                    tcgen05_commit(&empty[s]);
+                }
+        }
+    } else if (warp >= 4 && warp < 8) {
+        // ---- codes to bfloat16 in TMEM: a thread its row's 128 columns
+        const int quarter = warp & 3;
+        const uint32_t to = tmem_operands + (static_cast<uint32_t>(quarter * 32) << 16);
+        uint32_t i = 0;
+        bool ok = true;
+        for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step)
+            for (int chunk = c0; chunk < c1; ++chunk, ++i) {
+                const uint32_t s = i % STAGES, o = i % OPERANDS;
+                if (!mbar_wait_warp(&full[s], (i / STAGES) & 1, p.error, 45)) {
+                    ok = false;
+                    break;
+                }
+                const uint8_t* rec = smem + s * T::STAGE + T::X_BYTES + quarter * RECORD;
+                uint32_t w[4][4];                // [piece][word]
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<uint4*>(w[c]) = *reinterpret_cast<const uint4*>(rec + packed_word_at(lane, c));
+                float sc[GROUPS];
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g)
+                    sc[g] = to_f32(*reinterpret_cast<const __nv_bfloat16*>(rec + packed_scale_at(lane, g)));
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&empty[s]);
+                if (i >= OPERANDS && !mbar_wait_warp(&operand_empty[o], (i / OPERANDS - 1) & 1, p.error, 46)) {
+                    ok = false;
+                    break;
+                }
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g)
+                    scales[((i % PT_SCALE_SLOTS) * GROUPS + g) * PT_ROWS + quarter * 32 + lane] = sc[g];
+                tcgen05_fence_after();
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t v[32];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t word = w[c][2 * half + b];
+                            v[b * 16 + c * 4 + 0] = packed_bf16_pair<0>(word);
+                            v[b * 16 + c * 4 + 1] = packed_bf16_pair<1>(word);
+                            v[b * 16 + c * 4 + 2] = packed_bf16_pair<2>(word);
+                            v[b * 16 + c * 4 + 3] = packed_bf16_pair<3>(word);
+                        }
+                    tmem_store_32x32(to + o * 64 + half * 32, v);
+                }
+                tmem_store_wait();
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&operand_full[o]);
+            }
+    } else if (warp >= 8) {
+        // ---- group sums times scales
+        pdl_wait();
+        const int quarter = warp & 3, half = (warp - 8) >> 2;
+        const uint32_t from = tmem_sums + (static_cast<uint32_t>(quarter * 32) << 16) + half * COLS;
+        constexpr int LOAD = COLS < 32 ? COLS : 32;
+        uint32_t i = 0, a = 0;
+        bool ok = true;
+        for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step) {
+            uint64_t acc[COLS / 2];
+#pragma unroll
+            for (int j = 0; j < COLS / 2; ++j)
+                acc[j] = 0;
+            for (int chunk = c0; ok && chunk < c1; ++chunk, ++i)
+#pragma unroll 1
+                for (int g = 0; g < GROUPS; ++g, ++a) {
+                    const uint32_t d = a % SUMS;
+                    if (!mbar_wait_warp(&sums_full[d], (a / SUMS) & 1, p.error, 47)) {
+                        ok = false;
+                        break;
+                    }
+                    tcgen05_fence_after();
+                    const float s = scales[((i % PT_SCALE_SLOTS) * GROUPS + g) * PT_ROWS + quarter * 32 + lane];
+                    const uint64_t s2 = pair_of(s, s);
+#pragma unroll
+                    for (int col = 0; col < COLS; col += LOAD) {
+                        uint32_t v[LOAD];
+                        if constexpr (LOAD == 32)
+                            tmem_load_32x32(from + d * TOKENS + col, v);
+                        else
+                            tmem_load_32x16(from + d * TOKENS + col, v);
+                        tmem_load_wait();
+                        if (col + LOAD == COLS) {
+                            tcgen05_fence_before();
+                            __syncwarp();
+                            if (lane == 0)
+                                mbar_arrive(&sums_empty[d]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < LOAD / 2; ++j)
+                            acc[col / 2 + j] = pair_fma(s2, pair_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), acc[col / 2 + j]);
+                    }
+                }
+            if (!ok)
+                break;
+            if (p.splits > 1) {
+                // [column][row], where the stages were: all of this tile's copies and products are done, and there is one tile
+                float* mine = reinterpret_cast<float*>(smem) + half * COLS * PT_ROWS + quarter * 32 + lane;
+#pragma unroll
+                for (int j = 0; j < COLS / 2; ++j) {
+                    const float2 v = halves_of(acc[j]);
+                    mine[2 * j * PT_ROWS] = v.x;
+                    mine[(2 * j + 1) * PT_ROWS] = v.y;
+                }
+                continue;
+            }
+            const int token0 = tile % p.token_tiles * TOKENS + half * COLS, n_tile = tile / p.token_tiles;
+            if (p.pair) {
+                // lanes l and l ^ 8 hold a feature's gate and up: one makes the even tokens, the other the odd ones
+                const bool is_up = lane & 8;
+                const int at = n_tile * (PT_ROWS / 2) + quarter * 16 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+                for (int j = 0; j < COLS / 2; ++j) {
+                    const float2 v = halves_of(acc[j]);
+                    const float other = __shfl_xor_sync(0xffffffffu, is_up ? v.x : v.y, 8);
+                    const int token = token0 + 2 * j + (is_up ? 1 : 0);
+                    const float gate = is_up ? other : v.x, up = is_up ? v.y : other;
+                    if (token < p.m && at < p.n)
+                        packed_write(p, token, at, (p.out_type == CHIBI_F32 ? activate(gate, p.act) : activate_rounded(gate, p.act)) * up);
+                }
+            } else {
+                const int at = n_tile * PT_ROWS + quarter * 32 + lane;
+                if (at < p.n) {
+#pragma unroll
+                    for (int j0 = 0; j0 < COLS / 2; j0 += 4) {
+                        float r[8] = {};
+                        if (p.residual) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (token0 + 2 * j0 + j < p.m)
+                                    r[j] = p.residual[(long long)(token0 + 2 * j0 + j) * p.residual_stride + at];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 v = halves_of(acc[j0 + j]);
+                            const int token = token0 + 2 * (j0 + j);
+                            if (token < p.m)
+                                packed_write(p, token, at, v.x + r[2 * j]);
+                            if (token + 1 < p.m)
+                                packed_write(p, token + 1, at, v.y + r[2 * j + 1]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    __syncwarp();
+    if (p.splits > 1) {
+        pdl_wait();
+        __syncthreads();
+        cluster_sync();
+        // every CTA of the cluster adds up a share of the tile's columns, four rows a thread
+        const int token0 = first_tile % p.token_tiles * TOKENS, n_tile = first_tile / p.token_tiles;
+        const int tokens = min(TOKENS, p.m - token0);
+        const int t0 = tokens * rank / p.splits, t1 = tokens * (rank + 1) / p.splits;
+        const uint32_t base = smem_addr(smem);
+        for (int e = threadIdx.x; e < (t1 - t0) * (PT_ROWS / 4); e += PT_THREADS) {
+            const int token = t0 + e / (PT_ROWS / 4), row = e % (PT_ROWS / 4) * 4;
+            const bool up_rows = p.pair && (row & 8);
+            if (up_rows)
+                continue;
+            float v[4] = {}, up[4] = {};
+            for (int s = 0; s < p.splits; ++s) {
+                float part[4], up_part[4] = {};
+                peer_shared_f32x4(base + (token * PT_ROWS + row) * 4, s, part);
+                if (p.pair)
+                    peer_shared_f32x4(base + (token * PT_ROWS + row + 8) * 4, s, up_part);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] += part[j];
+                    up[j] += up_part[j];
+                }
+            }
+            const long long m = token0 + token;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = p.pair ? n_tile * (PT_ROWS / 2) + (row >> 4) * 8 + (row & 7) + j : n_tile * PT_ROWS + row + j;
+                if (at >= p.n)
+                    continue;
+                if (p.pair)
+                    v[j] = activate(v[j], p.act) * up[j];
+                else if (p.residual)
+                    v[j] += p.residual[m * p.residual_stride + at];
+                packed_write(p, m, at, v[j]);
+            }
+        }
+        __syncwarp();
+        cluster_sync();                          // nobody leaves while another reads
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem_sums, 512);
+    }
+}
+
+template <int TOKENS, int GROUP_BLOCKS>
+int launch_many_rows(const CUtensorMap& map, const PackedProduct& p, int ctas, cudaStream_t stream)
+{
+    constexpr size_t SMEM = PackedTile<TOKENS, GROUP_BLOCKS>::SMEM;
+    const cudaError_t e = cudaFuncSetAttribute(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)SMEM);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return (int)e;
+    }
+    launch_cluster_x(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, dim3((unsigned)ctas), dim3(PT_THREADS), SMEM, stream, p.splits, map, p);
+    return launch_status();
+}
+
+template <int TOKENS> int launch_many_rows_of(int group, const CUtensorMap& map, const PackedProduct& p, int ctas, cudaStream_t stream)
+{
+    return group == 32 ? launch_many_rows<TOKENS, 1>(map, p, ctas, stream)
+                       : (group == 64 ? launch_many_rows<TOKENS, 2>(map, p, ctas, stream) : launch_many_rows<TOKENS, 4>(map, p, ctas, stream));
+}
+
+} // namespace
+} // namespace chibi
+
+using namespace chibi;
+
+// out[m, n] = x[m, k] times the matrix (+ residual); pair: act(x gate) * (x up), n features.  `tokens`: rows of x of a tile;
+// `splits`: CTAs that share a tile's columns.  CHIBI_ERR_UNSUPPORTED where x's rows do not start on 16 bytes.
+CHIBI_API int chibi_packed_many_rows(const void* data, int group, int n, int k, int pair, const void* x, long long x_stride, int m, void* out,
+                                     int out_type, long long out_stride, const void* residual, long long residual_stride, int act,
+                                     int tokens, int splits, void* error, void* stream)
+{
+    if (!data || !x || !out || n < 1 || k < 1 || m < 1 || !packed_group_ok(group) || (out_type != CHIBI_F32 && out_type != CHIBI_BF16)
+        || (pair && (residual || (act != 1 && act != 2))))
+        return CHIBI_ERR_ARGUMENT;
+    const int chunks = (k + PACKED_COLS - 1) / PACKED_COLS;
+    if ((tokens != 32 && tokens != 64 && tokens != 128) || splits < 1 || splits > 8 || splits > chunks)
+        return CHIBI_ERR_ARGUMENT;
+    if ((reinterpret_cast<uintptr_t>(x) & 15) || x_stride % 8)
+        return CHIBI_ERR_UNSUPPORTED;
+    const int each = pair ? PACKED_ROWS / 2 : PACKED_ROWS, tile_rows = pair ? PT_ROWS / 2 : PT_ROWS;
+    const long long token_tiles = (m + (long long)tokens - 1) / tokens, tiles = (n + (long long)tile_rows - 1) / tile_rows * token_tiles;
+    if (tiles * splits > 0x7fffffff)
+        return CHIBI_ERR_UNSUPPORTED;
+    CUtensorMap map;
+    if (!tensor_map_2d(x, m, k, x_stride, tokens, &map))
+        return CHIBI_ERR_UNSUPPORTED;
+    const PackedProduct p { (const uint8_t*)data, (n + each - 1) / each, chunks, n, pair, m, out, out_type, out_stride, (const float*)residual,
+                            residual_stride, act, splits, (int)tiles, (int)token_tiles, (int*)error };
+    const int sms = device_sm_count();
+    const int ctas = splits > 1 ? (int)tiles * splits : (int)(tiles < sms ? tiles : sms);
+    return tokens == 32 ? launch_many_rows_of<32>(group, map, p, ctas, (cudaStream_t)stream)
+                        : (tokens == 64 ? launch_many_rows_of<64>(group, map, p, ctas, (cudaStream_t)stream)
+                                        : launch_many_rows_of<128>(group, map, p, ctas, (cudaStream_t)stream));
+}

@@ -4,6 +4,10 @@
 #include "packed.cuh"
 #include "sm100.cuh"
 
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
 namespace chibi {
 namespace {
 
@@ -32,7 +36,7 @@ __device__ __forceinline__ int nearest_code(float w, float s)
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(PackSource p, int row_blocks, int col_blocks, int group, uint8_t* out)
+__global__ void __launch_bounds__(512) pack_kernel(PackSource p, int row_blocks, int col_blocks, int group, uint8_t* out)
 {
     // (No pdl_trigger: products read their matrix before the kernel ahead of them has ended, so nothing may start before
     // this kernel has.)
@@ -41,8 +45,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackSource p, int row_blocks,
     const int lanes = group / 8;
     for (long long record = blockIdx.x; record < (long long)row_blocks * col_blocks; record += gridDim.x) {
         const int rb = (int)(record / col_blocks), cb = (int)(record % col_blocks);
-        const int side = p.pair ? r >> 3 : 0;
-        const int row = p.pair ? rb * 8 + (r & 7) : rb * PACKED_ROWS + r;
+        const int side = packed_side(p.pair, r), row = packed_source_row(p.pair, rb, r);
         const int col = cb * PACKED_COLS + seg * 8;
         float v[8];
         const T* src = static_cast<const T*>(p.w[side]) + (long long)row * p.stride[side] + col;
@@ -100,15 +103,14 @@ struct CodeSource {
     int rows, cols, pair;
 };
 
-__global__ void __launch_bounds__(256) pack_codes_kernel(CodeSource p, int row_blocks, int col_blocks, int group, uint8_t* out)
+__global__ void __launch_bounds__(512) pack_codes_kernel(CodeSource p, int row_blocks, int col_blocks, int group, uint8_t* out)
 {
     pdl_wait();
     const int r = threadIdx.x >> 4, seg = threadIdx.x & 15;
     const int lanes = group / 8;
     for (long long record = blockIdx.x; record < (long long)row_blocks * col_blocks; record += gridDim.x) {
         const int rb = (int)(record / col_blocks), cb = (int)(record % col_blocks);
-        const int side = p.pair ? r >> 3 : 0;
-        const int row = p.pair ? rb * 8 + (r & 7) : rb * PACKED_ROWS + r;
+        const int side = packed_side(p.pair, r), row = packed_source_row(p.pair, rb, r);
         const int col = cb * PACKED_COLS + seg * 8;
         uint32_t word = 0;
 #pragma unroll
@@ -126,21 +128,21 @@ __global__ void __launch_bounds__(256) pack_codes_kernel(CodeSource p, int row_b
 
 // The values, rows of a pair's first matrix before those of its second.
 template <typename T>
-__global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* data, int row_blocks, int col_blocks, int group, int rows, int cols,
+__global__ void __launch_bounds__(512) unpack_kernel(const uint8_t* data, int row_blocks, int col_blocks, int group, int rows, int cols,
                                                      int pair, T* out, long long stride)
 {
     pdl_enter();
     const int r = threadIdx.x >> 4, seg = threadIdx.x & 15;
     for (long long record = blockIdx.x; record < (long long)row_blocks * col_blocks; record += gridDim.x) {
         const int rb = (int)(record / col_blocks), cb = (int)(record % col_blocks);
-        const int row = pair ? rb * 8 + (r & 7) : rb * PACKED_ROWS + r;
+        const int row = packed_source_row(pair, rb, r);
         const int col = cb * PACKED_COLS + seg * 8;
         if (row >= rows || col >= cols)
             continue;
         const uint8_t* src = data + record * packed_record_bytes(group);
         const uint32_t word = *reinterpret_cast<const uint32_t*>(src + packed_word_at(r, seg));
         const float s = to_f32(*reinterpret_cast<const __nv_bfloat16*>(src + packed_scale_at(r, seg * 8 / group)));
-        T* dst = out + (long long)(row + (pair ? (r >> 3) * rows : 0)) * stride + col;
+        T* dst = out + (long long)(row + packed_side(pair, r) * rows) * stride + col;
         T v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -159,26 +161,28 @@ __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* data, int ro
 // ------------------------------------------------------------------ few rows of x
 // out[m][n] = sum over groups of s[n][g] * (sum over the group of q[n][k] x[m][k]).
 //
-// What bounds it is the bytes of the matrix.  A CTA of 16 warps stays on its SM; every warp streams records of its own
-// (bulk copies into a ring of its own, no barrier between warps), makes bfloat16 fragments of the codes and multiplies
-// them with x by `mma.m16n8k16`: the 16 rows of a record are the instruction's rows, 8 tokens its columns.  x lies in shared
-// memory as the fragments want it, 16 bytes to a lane for two instructions.  Each group's sums start at zero and are
+// What bounds it is the bytes of the matrix.  A CTA of 8 or 16 warps stays on its SM; every warp streams records of its own
+// (bulk copies into a ring of its own, no barrier between warps), makes float16 fragments of the codes and multiplies
+// them with x by `mma.m16n8k16`: 16 rows of a record are the instruction's rows, 8 tokens its columns.  x lies in shared
+// memory as the fragments want it, 16 bytes to a lane for four instructions.  Each group's sums start at zero and are
 // multiplied by the scales in 32 bits.
 //
-// 32-bit x is the sum of three bfloat16 numbers (its leading 8 bits, the next 8 and the last 8, cut off, not rounded, so that
-// the first does not overflow), three instructions for one.  Rows whose numbers in a CTA's columns are all small or some
-// very large are scaled by a power of two before and after, so that last parts are not lost below bfloat16's range and
-// sums over q x do not leave 32 bits where sums over s q x would not.
+// x becomes float16 too (two nibbles of a word are float16 numbers without a shift, which bfloat16's seven bits of mantissa
+// do not allow; the conversion of the codes is most of the kernel's instructions).  A row whose largest number of the CTA's
+// columns is not within 1 ... 2^15 is multiplied by the power of two that brings it to 2^14 ... 2^15, and its sums by the inverse: so
+// bfloat16 numbers from 2^-14 (of a scaled row: 2^-29 of the largest) on keep all of their bits, smaller ones are off by 2^-25 (2^-40) at
+// most.  32-bit numbers are two float16 numbers, the nearest and the nearest to what is left: off by 2^-23 of themselves or
+// by 2^-25 of the row's largest at most, no more than the 32-bit sums lose.
 //
 // How the work is shared out (CudaKernels.packed_plan chooses): `splits` CTAs of a cluster share the columns, `along_k`
-// warps of a CTA share the CTA's columns of one block of 16 rows, 16 / along_k blocks of rows are a unit, and clusters
+// warps of a CTA share the CTA's columns of one block of 32 rows, the CTA's warps / along_k blocks of rows are a unit, and clusters
 // take units in turn.  The sums of up to `batch` units stay in shared memory; then the cluster adds them up in one order
 // (CTA by CTA, warp by warp), each CTA a share of the outputs, so the same plan gives the same bits.
-constexpr int FEW_WARPS = 16, FEW_THREADS = FEW_WARPS * 32;
+constexpr int FEW_THREADS = 512;             // at most
 
 struct FewRows {
     const uint8_t* data;
-    int row_blocks, chunks;        // blocks of 16 rows, of 128 columns
+    int row_blocks, chunks;        // blocks of 32 rows, of 128 columns
     int n, k, pair;
     const void* x;
     long long x_stride;
@@ -189,16 +193,23 @@ struct FewRows {
     const float* residual;
     long long residual_stride;
     int act;                       // pairs: 1 gelu with tanh, 2 silu
-    int splits, along_k, batch, depth, tokens;     // tokens: rows of x of a CTA
+    int warps, splits, along_k, batch, depth, run, tokens;     // run: records of a stage; tokens: rows of x of a CTA
     int clusters;
     int* error;
 };
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+// FIRST: d is what comes out, else it is added to.
+template <bool FIRST> __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (FIRST) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+        return;
+    }
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ float peer_shared_f32(uint32_t own_smem_addr, uint32_t rank)
@@ -208,40 +219,48 @@ __device__ __forceinline__ float peer_shared_f32(uint32_t own_smem_addr, uint32_
     return v;
 }
 
-// The three parts of two 32-bit numbers, cut off: 8 + 8 + 8 bits, nothing lost above bfloat16's smallest number.  An infinity
-// or NaN is its first part alone.
-__device__ __forceinline__ void cut_parts(float a, float b, uint32_t (&parts)[3])
+// 8 neighbouring numbers of a row of x from column `col` on, zeros beyond its k columns.
+template <typename T> __device__ __forceinline__ void read_eight(const T* row, int col, int k, T (&v)[8])
 {
-    float r[2] = { a, b };
+    const T* src = row + col;
+    if (col + 8 <= k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        uint32_t top[2];
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src)[i];
+    } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t bits = __float_as_uint(r[j]);
-            // (a NaN whose upper half has no mantissa bit would turn into an infinity)
-            top[j] = i == 0 && isnan(r[j]) ? 0x7fc00000u : bits & 0xffff0000u;
-            r[j] = i == 0 && !isfinite(r[j]) ? 0.f : r[j] - __uint_as_float(top[j]);
-        }
-        parts[i] = (top[0] >> 16) | top[1];
+        for (int i = 0; i < 8; ++i)
+            v[i] = col + i < k ? src[i] : from_f32<T>(0.f);
     }
 }
 
-// The power of two by which a row of 32-bit numbers is multiplied, from the largest magnitude among its finite ones.
-__device__ __forceinline__ float row_factor(uint32_t largest_bits)
+// The exponent of the power of two by which a row is multiplied, from its largest finite magnitude: none where that is
+// 1 ... 2^15, else the one that brings it to 2^14 ... 2^15 (as far as a 32-bit number goes: rows below 2^-112 come out smaller).
+__device__ __forceinline__ int row_exponent(uint32_t largest_bits)
 {
-    const float v = __uint_as_float(largest_bits);
-    return v > 0x1p80f ? 0x1p-80f : (v < 0x1p-40f ? 0x1p80f : 1.f);
+    const int e = (int)(largest_bits >> 23) - 127;
+    return (e >= 0 && e < 15) || largest_bits == 0 ? 0 : min(14 - e, 126);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+
+// Two numbers as float16, and what is left of them (nothing of an infinity or NaN).
+__device__ __forceinline__ uint32_t take_half_pair(float (&v)[2])
+{
+    const __half2 h = __floats2half2_rn(v[0], v[1]);
+    v[0] = isfinite(v[0]) ? v[0] - __low2float(h) : 0.f;
+    v[1] = isfinite(v[1]) ? v[1] - __high2float(h) : 0.f;
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 template <int NT, bool X32, int GROUP_BLOCKS>
 __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows p)
 {
     using namespace sm100;
-    constexpr int PARTS = X32 ? 3 : 1;
+    using T = typename std::conditional<X32, float, __nv_bfloat16>::type;
+    constexpr int PARTS = X32 ? 2 : 1;
     constexpr int GROUPS = 4 / GROUP_BLOCKS;
-    constexpr int RECORD = PACKED_CODE_BYTES + GROUPS * 32;
-    constexpr int SUMS = 128 * NT;               // 32-bit sums of a warp
+    constexpr int RECORD = PACKED_CODE_BYTES + GROUPS * 64;
+    constexpr int SUMS = 256 * NT;               // 32-bit sums of a warp
     extern __shared__ __align__(1024) uint8_t smem[];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -251,115 +270,104 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows
     const int tokens = min(p.tokens, p.m - token0);
     const int c0 = (int)((long long)p.chunks * rank / p.splits), c1 = (int)((long long)p.chunks * (rank + 1) / p.splits);
     const int most = (p.chunks + p.splits - 1) / p.splits;
-    const int blocks_per_unit = FEW_WARPS / p.along_k;
+    const int blocks_per_unit = p.warps / p.along_k;
     const int units = (p.row_blocks + blocks_per_unit - 1) / blocks_per_unit;
 
-    // shared memory: rings | x | sums | row factors | barriers
+    // shared memory: rings | x | sums | the rows' largest numbers | barriers
     const uint32_t x_plane = (uint32_t)most * 4 * p.tokens * 64;
-    uint8_t* ring = smem + (size_t)warp * p.depth * RECORD;
-    uint8_t* xs = smem + (size_t)FEW_WARPS * p.depth * RECORD;
+    const int stage = p.run * RECORD;
+    uint8_t* ring = smem + warp * p.depth * stage;
+    uint8_t* xs = smem + p.warps * p.depth * stage;
     float* sums = reinterpret_cast<float*>(xs + (size_t)PARTS * x_plane);
-    uint32_t* largest = reinterpret_cast<uint32_t*>(sums + (size_t)p.batch * FEW_WARPS * SUMS);
-    uint64_t* full = reinterpret_cast<uint64_t*>(largest + 16 * NT) + warp * p.depth;
+    uint32_t* largest = reinterpret_cast<uint32_t*>(sums + p.batch * p.warps * SUMS);
+    uint64_t* full = reinterpret_cast<uint64_t*>(largest + 16) + warp * p.depth;
 
     // the warp's records: of its block of rows in every unit, columns w0 ... w1
     const int wk = warp % p.along_k, wr = warp / p.along_k;
-    const int w0 = c0 + (int)((long long)(c1 - c0) * wk / p.along_k), w1 = c0 + (int)((long long)(c1 - c0) * (wk + 1) / p.along_k);
+    const int w0 = c0 + (c1 - c0) * wk / p.along_k, w1 = c0 + (c1 - c0) * (wk + 1) / p.along_k;
     const int my_rounds = cluster < units ? (units - 1 - cluster) / p.clusters + 1 : 0;
     const int last_unit = cluster + (my_rounds - 1) * p.clusters;
     const int warp_rounds = my_rounds > 0 && last_unit * blocks_per_unit + wr >= p.row_blocks ? my_rounds - 1 : my_rounds;
-    const long long total = (long long)warp_rounds * (w1 - w0);
-    const long long round_step = (long long)p.clusters * blocks_per_unit * p.chunks * RECORD;
+    const long long round_step = ((long long)p.clusters * blocks_per_unit * p.chunks - (w1 - w0)) * RECORD;
     const uint8_t* next_src = p.data + ((long long)(cluster * blocks_per_unit + wr) * p.chunks + w0) * RECORD;
-    long long issued = 0;
-    int next_chunk = w0;
-    // (one lane)
+    int rounds_to_ask = w1 > w0 ? warp_rounds : 0, next_chunk = w0;
+    // asks for the next records of the warp, up to `run` of one block of rows
     auto issue = [&](int slot) {
-        mbar_arrive_expect_tx(&full[slot], RECORD);
-        bulk_load(ring + (size_t)slot * RECORD, next_src, RECORD, &full[slot]);
-    };
-    auto advance = [&]() {
-        ++issued;
-        next_src += RECORD;
-        if (++next_chunk == w1) {
+        const int bytes = min(p.run, w1 - next_chunk) * RECORD;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(&full[slot], bytes);
+            bulk_load(ring + slot * stage, next_src, bytes, &full[slot]);
+        }
+        next_src += bytes;
+        next_chunk += p.run;
+        if (next_chunk >= w1) {
             next_chunk = w0;
-            next_src += round_step - (long long)(w1 - w0) * RECORD;
+            next_src += round_step;
+            --rounds_to_ask;
         }
     };
     if (lane == 0)
         for (int i = 0; i < p.depth; ++i)
             mbar_init(&full[i], 1);
-    if (X32 && threadIdx.x < 16 * NT)
+    if (threadIdx.x < 16)
         largest[threadIdx.x] = 0;
     fence_barrier_init();
     fence_proxy_async();
-    __syncwarp();
-    for (int i = 0; i < p.depth && issued < total; ++i) {
-        if (lane == 0)
-            issue(i);
-        advance();
-    }
+    __syncthreads();
+    int open = 0;                                // stages that were asked for and not waited for
+    for (; open < p.depth && rounds_to_ask > 0; ++open)
+        issue(open);
 
     // ---- x as fragments: [block of 32 columns][token][lane % 4], 8 neighbouring columns each
     pdl_wait();
-    const int pieces = (c1 - c0) * 16 * tokens;
-    auto read_piece = [&](int i, float (&v)[8]) -> uint32_t {
-        // neighbouring threads take neighbouring pieces of a token; returns where the piece goes
-        const int token = i / ((c1 - c0) * 16), seg = i % ((c1 - c0) * 16);
-        const int col = c0 * PACKED_COLS + seg * 8;
-        if constexpr (X32) {
-            const float* src = static_cast<const float*>(p.x) + (long long)(token0 + token) * p.x_stride + col;
-            if (col + 8 <= p.k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-                *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(src + 4);
-            } else {
+    // (warps / tokens warps to a token)
+    const int token_pieces = (c1 - c0) * 16, token_warps = p.warps / tokens;
+    const int token = warp % tokens, first_piece = warp / tokens < token_warps ? (warp / tokens) * 32 + lane : token_pieces;
+    const T* x_row = static_cast<const T*>(p.x) + (token0 + token) * p.x_stride;
+    auto put = [&](int i, const T (&raw)[8], float up_by) {
+        float pairs[4][2];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    v[j] = col + j < p.k ? src[j] : 0.f;
-            }
-        }
-        return (uint32_t)(((seg >> 2) * p.tokens + token) * 64 + (seg & 3) * 16);
+        for (int j = 0; j < 8; ++j)
+            pairs[j / 2][j % 2] = to_f32(raw[j]) * up_by;
+        uint8_t* dst = xs + ((i >> 2) * p.tokens + token) * 64 + (i & 3) * 16;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+            *reinterpret_cast<uint4*>(dst + part * x_plane)
+                = make_uint4(take_half_pair(pairs[0]), take_half_pair(pairs[1]), take_half_pair(pairs[2]), take_half_pair(pairs[3]));
     };
-    if constexpr (X32) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < pieces; i += FEW_THREADS) {
-            float v[8];
-            read_piece(i, v);
-            float most_of = 0.f;
+    // once as it is (and rows that want a factor once more)
+    constexpr int AT_ONCE = X32 ? 4 : 8;         // pieces of a thread on their way
+    float most_of = 0.f;
+    for (int i0 = first_piece; i0 < token_pieces; i0 += AT_ONCE * token_warps * 32) {
+        T raw[AT_ONCE][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                most_of = isfinite(v[j]) ? fmaxf(most_of, fabsf(v[j])) : most_of;
-            atomicMax(&largest[i / ((c1 - c0) * 16)], __float_as_uint(most_of));
+        for (int a = 0; a < AT_ONCE; ++a) {
+            const int i = i0 + a * token_warps * 32;
+            if (i < token_pieces)
+                read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw[a]);
         }
-        __syncthreads();
-    }
-    for (int i = threadIdx.x; i < pieces; i += FEW_THREADS) {
-        float v[8];
-        const uint32_t at = read_piece(i, v);
-        if constexpr (X32) {
-            const float f = row_factor(largest[i / ((c1 - c0) * 16)]);
-            uint32_t parts[4][3];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                cut_parts(v[2 * j] * f, v[2 * j + 1] * f, parts[j]);
+        for (int a = 0; a < AT_ONCE; ++a) {
+            const int i = i0 + a * token_warps * 32;
+            if (i < token_pieces) {
 #pragma unroll
-            for (int part = 0; part < 3; ++part)
-                *reinterpret_cast<uint4*>(xs + part * x_plane + at) = make_uint4(parts[0][part], parts[1][part], parts[2][part], parts[3][part]);
-        } else {
-            const int token = i / ((c1 - c0) * 16), seg = i % ((c1 - c0) * 16);
-            const int col = c0 * PACKED_COLS + seg * 8;
-            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.x) + (long long)(token0 + token) * p.x_stride + col;
-            uint4 w;
-            if (col + 8 <= p.k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                w = *reinterpret_cast<const uint4*>(src);
-            } else {
-                uint32_t h[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    h[j] = col + j < p.k ? (uint32_t)__bfloat16_as_ushort(src[j]) : 0u;
-                w = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                for (int j = 0; j < 8; ++j) {
+                    const float v = fabsf(to_f32(raw[a][j]));
+                    most_of = v < INFINITY ? fmaxf(most_of, v) : most_of;
+                }
+                put(i, raw[a], 1.f);
             }
-            *reinterpret_cast<uint4*>(xs + at) = w;
+        }
+    }
+    const uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
+    if (lane == 0)
+        atomicMax(&largest[token], warps_most);
+    __syncthreads();
+    if (const int e = row_exponent(largest[token])) {
+        for (int i = first_piece; i < token_pieces; i += token_warps * 32) {
+            T raw[8];
+            read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
+            put(i, raw, power_of_two(e));
         }
     }
     __syncthreads();
@@ -371,90 +379,104 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows
     float down[NT][2];                           // undo the rows' factors
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        x_lane[t] = smem_addr(xs) + (uint32_t)min(t * 8 + r, tokens - 1) * 64 + c * 16;
+        x_lane[t] = (uint32_t)min(t * 8 + r, tokens - 1) * 64 + c * 16;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            down[t][j] = X32 ? 1.f / row_factor(largest[min(t * 8 + 2 * c + j, tokens - 1)]) : 1.f;
+            down[t][j] = power_of_two(-row_exponent(largest[min(t * 8 + 2 * c + j, tokens - 1)]));
     }
     const uint32_t x_block = (uint32_t)p.tokens * 64;
-    bool dead = false;                           // a wait ran out: nothing more is asked for or computed
+    bool dead = false;                           // a wait ran out: nothing more is asked for
     int slot = 0;
     uint32_t phase = 0;
-    long long taken = 0;
 
     for (int first = 0; first < my_rounds; first += p.batch) {
         const int now = min(p.batch, my_rounds - first);
         for (int u = 0; u < now; ++u) {
-            float acc[NT][4];
+            float acc[2][NT][4];
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-            const int todo = first + u < warp_rounds ? w1 - w0 : 0;
-            for (int j = 0; j < todo; ++j) {
-                if (!dead || taken < issued)
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    acc[h][t][0] = acc[h][t][1] = acc[h][t][2] = acc[h][t][3] = 0.f;
+            int todo = first + u < warp_rounds ? w1 - w0 : 0;
+            const uint8_t* x_at = xs + (w0 - c0) * 4 * x_block;
+            while (todo > 0) {
+                if (open > 0) {
                     dead = !mbar_wait_warp(&full[slot], phase, p.error, 41) || dead;
-                ++taken;
-                const uint8_t* rec = ring + (size_t)slot * RECORD;
-                const uint4 lo = *reinterpret_cast<const uint4*>(rec + code_at);
-                const uint4 hi = *reinterpret_cast<const uint4*>(rec + code_at + 512);
-                uint32_t scale[GROUPS];
+                    --open;
+                }
+                const uint8_t* rec = ring + slot * stage + code_at;
+                const uint8_t* rec_scales = ring + slot * stage + PACKED_CODE_BYTES + r * 8;
+                const int here = min(todo, p.run);
+                todo -= here;
+                for (int j = 0; j < here; ++j, rec += RECORD, rec_scales += RECORD, x_at += 4 * x_block) {
+                    uint32_t w[4][4];                        // rows r, r + 8, r + 16, r + 24
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g)
-                    scale[g] = *reinterpret_cast<const uint32_t*>(rec + PACKED_CODE_BYTES + g * 32 + r * 4);
-                __syncwarp();
-                if (!dead && issued < total) {
-                    if (lane == 0)
-                        issue(slot);
-                    advance();
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(rec + i * 512);
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g) {
+                        const uint2 s = *reinterpret_cast<const uint2*>(rec_scales + g * 64);
+                        float d[2][NT][4];
+#pragma unroll
+                        for (int i = 0; i < GROUP_BLOCKS; ++i) {
+                            const int b = g * GROUP_BLOCKS + i;
+                            uint4 f[PARTS][NT];
+#pragma unroll
+                            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                                for (int t = 0; t < NT; ++t)
+                                    f[part][t] = *reinterpret_cast<const uint4*>(x_at + x_lane[t] + b * x_block + part * x_plane);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t q0[4], q1[4];
+                                packed_half_pairs(w[2 * h][b], q0);
+                                packed_half_pairs(w[2 * h + 1][b], q1);
+                                const uint32_t a0[4] = { q0[0], q1[0], q0[1], q1[1] }, a1[4] = { q0[2], q1[2], q0[3], q1[3] };
+#pragma unroll
+                                for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                                    for (int t = 0; t < NT; ++t) {
+                                        if (i == 0 && part == 0)
+                                            mma_16816<true>(d[h][t], a0, f[part][t].x, f[part][t].y);
+                                        else
+                                            mma_16816<false>(d[h][t], a0, f[part][t].x, f[part][t].y);
+                                        mma_16816<false>(d[h][t], a1, f[part][t].z, f[part][t].w);
+                                    }
+                            }
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t two = h ? s.y : s.x;
+                            const float s0 = __uint_as_float(two << 16), s1 = __uint_as_float(two & 0xffff0000u);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                acc[h][t][0] = fmaf(s0, d[h][t][0], acc[h][t][0]);
+                                acc[h][t][1] = fmaf(s0, d[h][t][1], acc[h][t][1]);
+                                acc[h][t][2] = fmaf(s1, d[h][t][2], acc[h][t][2]);
+                                acc[h][t][3] = fmaf(s1, d[h][t][3], acc[h][t][3]);
+                            }
+                        }
+                    }
+                }
+                __syncwarp();                    // all lanes have read the stage
+                if (!dead && rounds_to_ask > 0) {
+                    issue(slot);
+                    ++open;
                 }
                 if (++slot == p.depth) {
                     slot = 0;
                     phase ^= 1;
                 }
-                const uint32_t words[2][4] = { { lo.x, lo.y, lo.z, lo.w }, { hi.x, hi.y, hi.z, hi.w } };
-                const uint32_t x_at = (uint32_t)(w0 - c0 + j) * 4 * x_block;
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    float d[NT][4];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        d[t][0] = d[t][1] = d[t][2] = d[t][3] = 0.f;
-#pragma unroll
-                    for (int i = 0; i < GROUP_BLOCKS; ++i) {
-                        const int b = g * GROUP_BLOCKS + i;
-                        const uint32_t a0[4] = { packed_pair<0>(words[0][b]), packed_pair<0>(words[1][b]),
-                                                 packed_pair<1>(words[0][b]), packed_pair<1>(words[1][b]) };
-                        const uint32_t a1[4] = { packed_pair<2>(words[0][b]), packed_pair<2>(words[1][b]),
-                                                 packed_pair<3>(words[0][b]), packed_pair<3>(words[1][b]) };
-#pragma unroll
-                        for (int part = 0; part < PARTS; ++part) {
-#pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                uint4 f;
-                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                             : "=r"(f.x), "=r"(f.y), "=r"(f.z), "=r"(f.w)
-                                             : "r"(x_lane[t] + x_at + b * x_block + part * x_plane));
-                                mma_16816(d[t], a0, f.x, f.y);
-                                mma_16816(d[t], a1, f.z, f.w);
-                            }
-                        }
-                    }
-                    const float s0 = __uint_as_float(scale[g] << 16), s1 = __uint_as_float(scale[g] & 0xffff0000u);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        acc[t][0] = fmaf(s0, d[t][0], acc[t][0]);
-                        acc[t][1] = fmaf(s0, d[t][1], acc[t][1]);
-                        acc[t][2] = fmaf(s1, d[t][2], acc[t][2]);
-                        acc[t][3] = fmaf(s1, d[t][3], acc[t][3]);
-                    }
-                }
             }
-            float* mine = sums + ((size_t)u * FEW_WARPS + warp) * SUMS + lane;
+            float* mine = sums + (u * p.warps + warp) * SUMS + lane;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    mine[(t * 4 + e) * 32] = acc[t][e] * down[t][e & 1];
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mine[((h * NT + t) * 4 + e) * 32] = acc[h][t][e] * down[t][e & 1];
         }
 
         // ---- the cluster adds up what its warps have
@@ -463,28 +485,37 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows
             cluster_sync();
         else
             __syncthreads();
-        const int rows_out = p.pair ? 8 : 16;
+        const int rows_out = p.pair ? PACKED_ROWS / 2 : PACKED_ROWS;
         const int outputs = now * blocks_per_unit * rows_out * tokens;
-        for (int e = rank * FEW_THREADS + threadIdx.x; e < outputs; e += p.splits * FEW_THREADS) {
+        for (int e = rank * blockDim.x + threadIdx.x; e < outputs; e += p.splits * blockDim.x) {
             const int row = e % rows_out;
             const int token = e / rows_out % tokens;
             const int block = e / (rows_out * tokens);                   // of the batch: unit by unit
             const int u = block / blocks_per_unit, b = block % blocks_per_unit;
-            const int rb = (cluster + (first + u) * p.clusters) * blocks_per_unit + b;
-            const int at = rb * rows_out + row;
+            const int at = ((cluster + (first + u) * p.clusters) * blocks_per_unit + b) * rows_out + row;
             if (at >= p.n)
                 continue;
-            // the fragment's place of (row, token)
-            const int reg = (token >> 3) * 4 + (row >> 3) * 2 + (token & 1);
-            const uint32_t place = smem_addr(sums + ((size_t)u * FEW_WARPS + b * p.along_k) * SUMS + reg * 32 + (row & 7) * 4 + (token & 7) / 2);
+            // the fragment's place of (row of the record, token); a pair's up lies two registers behind its gate
+            const int in_record = p.pair ? (row >> 3) * 16 + (row & 7) : row;
+            const int reg = ((in_record >> 4) * NT + (token >> 3)) * 4 + ((in_record >> 3) & 1) * 2 + (token & 1);
+            const float* place = sums + (u * p.warps + b * p.along_k) * SUMS + reg * 32 + (in_record & 7) * 4 + (token & 7) / 2;
             float v = 0.f, up = 0.f;
-            for (int s = 0; s < p.splits; ++s)
+            if (p.splits > 1) {
+                const uint32_t from = smem_addr(place);
+                for (int s = 0; s < p.splits; ++s)
+                    for (int w = 0; w < p.along_k; ++w) {
+                        v += peer_shared_f32(from + w * (SUMS * 4), s);
+                        if (p.pair)
+                            up += peer_shared_f32(from + w * (SUMS * 4) + 256, s);
+                    }
+            } else {
+#pragma unroll 4
                 for (int w = 0; w < p.along_k; ++w) {
-                    const uint32_t from = place + (uint32_t)w * SUMS * 4;
-                    v += p.splits > 1 ? peer_shared_f32(from, s) : *reinterpret_cast<const float*>(__cvta_shared_to_generic(from));
+                    v += place[w * SUMS];
                     if (p.pair)
-                        up += p.splits > 1 ? peer_shared_f32(from + 256, s) : *reinterpret_cast<const float*>(__cvta_shared_to_generic(from + 256));
+                        up += place[w * SUMS + 64];
                 }
+            }
             if (p.pair)
                 v = activate(v, p.act) * up;
             const long long m = token0 + token;
@@ -512,11 +543,17 @@ void (*few_rows_kernel_of(int group))(FewRows)
 
 constexpr size_t FEW_SMEM_LIMIT = 227 * 1024;
 
-size_t few_rows_smem(int nt, bool x32, int group, int chunks, int splits, int batch, int depth, int tokens)
+size_t few_rows_smem(bool x32, int group, int chunks, int warps, int splits, int batch, int depth, int run, int tokens)
 {
     const size_t x_plane = (size_t)((chunks + splits - 1) / splits) * 4 * tokens * 64;
-    return (size_t)FEW_WARPS * depth * packed_record_bytes(group) + (x32 ? 3 : 1) * x_plane
-        + (size_t)batch * FEW_WARPS * 128 * nt * 4 + 16 * nt * 4 + FEW_WARPS * depth * 8;
+    return (size_t)warps * depth * run * packed_record_bytes(group) + (x32 ? 2 : 1) * x_plane
+        + (size_t)batch * warps * 256 * (tokens <= 8 ? 1 : 2) * 4 + 16 * 4 + warps * depth * 8;
+}
+
+void (*few_rows_kernel(bool x32, int tokens, int group))(FewRows)
+{
+    return x32 ? (tokens <= 8 ? few_rows_kernel_of<1, true>(group) : few_rows_kernel_of<2, true>(group))
+               : (tokens <= 8 ? few_rows_kernel_of<1, false>(group) : few_rows_kernel_of<2, false>(group));
 }
 
 } // namespace
@@ -531,10 +568,10 @@ CHIBI_API int chibi_pack_weights(const void* w, const void* up, int type, int ro
     if (!w || !out || rows < 1 || cols < 1 || !packed_group_ok(group))
         return CHIBI_ERR_ARGUMENT;
     const PackSource src { { w, up }, { stride, up_stride }, rows, cols, up ? 1 : 0 };
-    const int each = up ? 8 : PACKED_ROWS;
+    const int each = up ? PACKED_ROWS / 2 : PACKED_ROWS;
     const int row_blocks = (rows + each - 1) / each, col_blocks = (cols + PACKED_COLS - 1) / PACKED_COLS;
     const long long records = (long long)row_blocks * col_blocks;
-    CHIBI_DISPATCH_TYPE(type, T, launch(pack_kernel<T>, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(256), 0,
+    CHIBI_DISPATCH_TYPE(type, T, launch(pack_kernel<T>, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(512), 0,
                                         (cudaStream_t)stream, src, row_blocks, col_blocks, group, (uint8_t*)out));
     return launch_status();
 }
@@ -548,10 +585,10 @@ CHIBI_API int chibi_pack_codes(const void* codes, const void* scales, const void
     const CodeSource src { { (const int8_t*)codes, (const int8_t*)up_codes },
                            { (const __nv_bfloat16*)scales, (const __nv_bfloat16*)up_scales },
                            { stride, up_stride }, { scale_stride, up_scale_stride }, rows, cols, up_codes ? 1 : 0 };
-    const int each = up_codes ? 8 : PACKED_ROWS;
+    const int each = up_codes ? PACKED_ROWS / 2 : PACKED_ROWS;
     const int row_blocks = (rows + each - 1) / each, col_blocks = (cols + PACKED_COLS - 1) / PACKED_COLS;
     const long long records = (long long)row_blocks * col_blocks;
-    launch(pack_codes_kernel, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(256), 0, (cudaStream_t)stream, src, row_blocks,
+    launch(pack_codes_kernel, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(512), 0, (cudaStream_t)stream, src, row_blocks,
            col_blocks, group, (uint8_t*)out);
     return launch_status();
 }
@@ -561,33 +598,31 @@ CHIBI_API int chibi_unpack_weights(const void* data, int rows, int cols, int pai
 {
     if (!data || !out || rows < 1 || cols < 1 || !packed_group_ok(group))
         return CHIBI_ERR_ARGUMENT;
-    const int each = pair ? 8 : PACKED_ROWS;
+    const int each = pair ? PACKED_ROWS / 2 : PACKED_ROWS;
     const int row_blocks = (rows + each - 1) / each, col_blocks = (cols + PACKED_COLS - 1) / PACKED_COLS;
     const long long records = (long long)row_blocks * col_blocks;
-    CHIBI_DISPATCH_TYPE(out_type, T, launch(unpack_kernel<T>, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(256), 0,
+    CHIBI_DISPATCH_TYPE(out_type, T, launch(unpack_kernel<T>, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(512), 0,
                                             (cudaStream_t)stream, (const uint8_t*)data, row_blocks, col_blocks, group, rows, cols, pair,
                                             (T*)out, stride));
     return launch_status();
 }
 
 // Shared memory of the kernel for few rows under a plan, in KB (rounded up); CudaKernels.packed_plan asks.
-CHIBI_API int chibi_packed_few_rows_kb(int x32, int group, int cols, int tokens, int splits, int batch, int depth)
+CHIBI_API int chibi_packed_few_rows_kb(int x32, int group, int cols, int tokens, int warps, int splits, int batch, int depth, int run)
 {
-    const int nt = tokens <= 8 ? 1 : 2;
-    return (int)((few_rows_smem(nt, x32 != 0, group, (cols + PACKED_COLS - 1) / PACKED_COLS, splits, batch, depth, tokens) + 1023) / 1024);
+    return (int)((few_rows_smem(x32 != 0, group, (cols + PACKED_COLS - 1) / PACKED_COLS, warps, splits, batch, depth, run, tokens) + 1023)
+                 / 1024);
 }
 
 // How many clusters of `splits` CTAs with that much shared memory run at once (0: none, or an error).
-CHIBI_API int chibi_packed_few_rows_clusters(int x32, int group, int tokens, int splits, int kb)
+CHIBI_API int chibi_packed_few_rows_clusters(int x32, int group, int tokens, int warps, int splits, int kb)
 {
-    if (!packed_group_ok(group) || splits < 1 || splits > 8 || tokens < 1 || tokens > 16 || kb < 1 || kb > 227)
+    if (!packed_group_ok(group) || splits < 1 || splits > 8 || tokens < 1 || tokens > 16 || kb < 1 || kb > 227 || warps < 1 || warps > 16)
         return 0;
-    const int nt = tokens <= 8 ? 1 : 2;
-    void (*kernel)(FewRows) = x32 ? (nt == 1 ? few_rows_kernel_of<1, true>(group) : few_rows_kernel_of<2, true>(group))
-                                  : (nt == 1 ? few_rows_kernel_of<1, false>(group) : few_rows_kernel_of<2, false>(group));
+    void (*kernel)(FewRows) = few_rows_kernel(x32 != 0, tokens, group);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)splits);
-    cfg.blockDim = dim3(FEW_THREADS);
+    cfg.blockDim = dim3((unsigned)warps * 32);
     cfg.dynamicSmemBytes = (size_t)kb * 1024;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -607,33 +642,31 @@ CHIBI_API int chibi_packed_few_rows_clusters(int x32, int group, int tokens, int
 // out[m, n] = x[m, k] times the matrix (+ residual); pair: act(x gate) * (x up), n features.  The plan: see FewRows.
 CHIBI_API int chibi_packed_few_rows(const void* data, int group, int n, int k, int pair, const void* x, int x_type, long long x_stride,
                                     int m, void* out, int out_type, long long out_stride, const void* residual,
-                                    long long residual_stride, int act, int splits, int along_k, int batch, int depth, int tokens,
-                                    int clusters, void* error, void* stream)
+                                    long long residual_stride, int act, int warps, int splits, int along_k, int batch, int depth, int run,
+                                    int tokens, int clusters, void* error, void* stream)
 {
     if (!data || !x || !out || n < 1 || k < 1 || m < 1 || !packed_group_ok(group) || (x_type != CHIBI_F32 && x_type != CHIBI_BF16)
         || (out_type != CHIBI_F32 && out_type != CHIBI_BF16) || (pair && (residual || (act != 1 && act != 2))))
         return CHIBI_ERR_ARGUMENT;
     const int chunks = (k + PACKED_COLS - 1) / PACKED_COLS;
-    if (splits < 1 || splits > 8 || (splits & (splits - 1)) || splits > chunks || along_k < 1 || along_k > FEW_WARPS
-        || (along_k & (along_k - 1)) || batch < 1 || depth < 1 || tokens < 1 || tokens > 16 || clusters < 1)
+    if ((warps != 8 && warps != 16) || splits < 1 || splits > 8 || (splits & (splits - 1)) || splits > chunks || along_k < 1
+        || along_k > warps || (along_k & (along_k - 1)) || batch < 1 || depth < 1 || run < 1 || tokens < 1 || tokens > warps || clusters < 1)
         return CHIBI_ERR_ARGUMENT;
-    const int nt = tokens <= 8 ? 1 : 2;
     const bool x32 = x_type == CHIBI_F32;
-    const size_t smem = few_rows_smem(nt, x32, group, chunks, splits, batch, depth, tokens);
+    const size_t smem = few_rows_smem(x32, group, chunks, warps, splits, batch, depth, run, tokens);
     const long long token_blocks = ((long long)m + tokens - 1) / tokens;
+    const int each = pair ? PACKED_ROWS / 2 : PACKED_ROWS;
     if (smem > FEW_SMEM_LIMIT || token_blocks > 65535)
         return CHIBI_ERR_UNSUPPORTED;
-    const int each = pair ? 8 : PACKED_ROWS;
     const FewRows p { (const uint8_t*)data, (n + each - 1) / each, chunks, n, k, pair, x, x_stride, m, out, out_type, out_stride,
-                      (const float*)residual, residual_stride, act, splits, along_k, batch, depth, tokens, clusters, (int*)error };
-    void (*kernel)(FewRows) = x32 ? (nt == 1 ? few_rows_kernel_of<1, true>(group) : few_rows_kernel_of<2, true>(group))
-                                  : (nt == 1 ? few_rows_kernel_of<1, false>(group) : few_rows_kernel_of<2, false>(group));
+                      (const float*)residual, residual_stride, act, warps, splits, along_k, batch, depth, run, tokens, clusters, (int*)error };
+    void (*kernel)(FewRows) = few_rows_kernel(x32, tokens, group);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SMEM_LIMIT);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return (int)e;
     }
-    launch_cluster_x(kernel, dim3((unsigned)(clusters * splits), (unsigned)token_blocks), dim3(FEW_THREADS), smem, (cudaStream_t)stream,
-                     splits, p);
+    launch_cluster_x(kernel, dim3((unsigned)(clusters * splits), (unsigned)token_blocks), dim3((unsigned)warps * 32), smem,
+                     (cudaStream_t)stream, splits, p);
     return launch_status();
 }

@@ -14,7 +14,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import library
-from .packed import GROUPS, FewRowsPlan, PackedWeights, few_rows_plan
+from .packed import GROUPS, FewRowsPlan, PackedWeights, few_rows_plan, many_rows_cut
 from ..csrc import build
 
 F32, BF16 = 0, 1
@@ -179,6 +179,8 @@ class CudaKernels:
         self._attention_tc_libs = {}
         self._attention_tied_libs = {}
         self.use_tcgen05_attention = True
+        # matrices in 4 bits: up to so many bfloat16 rows of x stream the matrix once through mma.sync, more go to tcgen05
+        self.packed_few_rows_max = 16
         self._packed_plans: Dict[tuple, FewRowsPlan] = {}
         self._partial_bufs = [None, None]
         self._partial_turn = 0
@@ -469,6 +471,9 @@ class CudaKernels:
                     33: "a wait that ran out (experts' product: epilogue)",
                     34: "a wait that ran out (experts' product: accumulator hand-over)",
                     41: "a wait that ran out (product with a matrix in 4 bits: few rows)",
+                    **{c: f"a wait that ran out (product with a matrix in 4 bits: {w})" for c, w in
+                       ((42, "loader"), (43, "tensor-core issuer"), (44, "accumulator hand-over"), (45, "converting warps"),
+                        (46, "operand hand-over"), (47, "adding warps"))},
                     **{c: f"a wait that ran out (tcgen05 attention, point {c})" for c in range(21, 30)}}.get(code, f"code {code}")
             raise KernelError(f"a kernel refused {what}")
 
@@ -870,8 +875,8 @@ class CudaKernels:
         if plan is None:
             lib, x = self.lib, int(x32)
             plan = few_rows_plan(w.rows, w.columns, w.paired, m,
-                                 lambda tokens, splits, batch, depth: lib.chibi_packed_few_rows_kb(x, w.group, w.columns, tokens, splits, batch, depth),
-                                 lambda tokens, splits, kb: lib.chibi_packed_few_rows_clusters(x, w.group, tokens, splits, kb))
+                                 lambda *cut: lib.chibi_packed_few_rows_kb(x, w.group, w.columns, *cut),
+                                 lambda *cut: lib.chibi_packed_few_rows_clusters(x, w.group, *cut))
             if plan is None:
                 raise KernelError(f"a product over {w.columns} columns in 4 bits: more than the kernel holds")
             if len(self._packed_plans) > 4096:
@@ -899,13 +904,23 @@ class CudaKernels:
         if M == 0:
             return
         with self._current_device():
+            if x_code == BF16 and M > self.packed_few_rows_max:
+                status = self.lib.chibi_packed_many_rows(
+                    _ptr(w.data), w.group, w.rows, w.columns, int(w.paired), _ptr(x), x.stride(0), M, _ptr(out), out_code, out.stride(0),
+                    _ptr(residual), residual.stride(0) if residual is not None else 0, self.ACTIVATIONS[kind] if kind else 0,
+                    *many_rows_cut(w.rows, w.columns, w.paired, M, self.sm_count), _ptr(self.error), self._stream())
+                if status != -2:
+                    _check(status, what)
+                    self.launches += 1
+                    self.tensor_core_calls += 1
+                    return
             plan = self.packed_plan(w, M, x_code == F32)
             self.launches += 1
             self.tensor_core_calls += 1
             _check(self.lib.chibi_packed_few_rows(
                 _ptr(w.data), w.group, w.rows, w.columns, int(w.paired), _ptr(x), x_code, x.stride(0), M, _ptr(out), out_code, out.stride(0),
                 _ptr(residual), residual.stride(0) if residual is not None else 0, self.ACTIVATIONS[kind] if kind else 0,
-                plan.splits, plan.along_k, plan.batch, plan.depth, plan.tokens, plan.clusters, _ptr(self.error), self._stream()), what)
+                *plan, _ptr(self.error), self._stream()), what)
 
     def qk_norm_rope_append(self, qkv: torch.Tensor, q_out: torch.Tensor,
                             k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],

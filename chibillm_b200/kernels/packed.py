@@ -7,13 +7,12 @@ src/tensor/matrix.h:32-108).
 """
 from __future__ import annotations
 
-from typing import Callable, NamedTuple, Optional
+from typing import Callable, NamedTuple, Optional, Tuple
 
 import torch
 
 GROUPS = (32, 64, 128)
-BLOCK_ROWS, BLOCK_COLS = 16, 128
-FEW_WARPS = 16                    # warps of a CTA of the product with few rows
+BLOCK_ROWS, BLOCK_COLS = 32, 128
 FEW_TOKENS = 16                   # rows of x that such a CTA takes at most
 FEW_SMEM_KB = 227
 
@@ -44,51 +43,66 @@ class PackedWeights:
 
 class FewRowsPlan(NamedTuple):
     """See FewRows in csrc/packed_weights.cu."""
+    warps: int
     splits: int
     along_k: int
     batch: int
     depth: int
+    run: int
     tokens: int
     clusters: int
 
 
-def few_rows_plan(rows: int, columns: int, paired: bool, m: int, smem_kb: Callable[[int, int, int, int], int],
-                  most_clusters: Callable[[int, int, int], int]) -> Optional[FewRowsPlan]:
-    """How CTAs and warps share a product of m rows of x.  ``smem_kb(tokens, splits, batch, depth)`` is a CTA's shared
-    memory, ``most_clusters(tokens, splits, kb)`` how many clusters run at once.  None if nothing fits."""
+def few_rows_plan(rows: int, columns: int, paired: bool, m: int, smem_kb: Callable[..., int],
+                  most_clusters: Callable[[int, int, int, int], int]) -> Optional[FewRowsPlan]:
+    """How CTAs and warps share a product of m rows of x.  ``smem_kb(tokens, warps, splits, batch, depth, run)`` is a CTA's
+    shared memory, ``most_clusters(tokens, warps, splits, kb)`` how many clusters run at once.  None if nothing fits."""
     blocks = -(-rows // (BLOCK_ROWS // 2 if paired else BLOCK_ROWS))
     chunks = -(-columns // BLOCK_COLS)
     tokens = -(-m // -(-m // FEW_TOKENS))
     while tokens >= 1:
         best = None
         token_blocks = -(-m // tokens)
-        for splits in (1, 2, 4, 8):
-            if splits > chunks:
-                break
-            mine = -(-chunks // splits)
-            for depth in (4, 3, 2):
-                if smem_kb(tokens, splits, 1, depth) <= FEW_SMEM_KB:
+        for warps, room in ((8, FEW_SMEM_KB // 2), (16, FEW_SMEM_KB)):
+            if tokens > warps:
+                continue
+            for splits in (1, 2, 4, 8):
+                if splits > chunks:
                     break
-            else:
-                continue
-            at_once = most_clusters(tokens, splits, smem_kb(tokens, splits, 1, depth))
-            if at_once < 1:
-                continue
-            for along_k in (16, 8, 4, 2, 1):
-                if along_k > 1 and along_k // 2 >= mine:
-                    continue                     # half of the warps would have nothing
-                per_unit = FEW_WARPS // along_k
-                units = -(-blocks // per_unit)
-                clusters = min(units, max(1, at_once // token_blocks))
-                rounds = -(-units // clusters)
-                cost = rounds * (per_unit * mine + 2) + (20 if splits > 1 else 0)
-                if best is None or cost < best[0]:
-                    best = (cost, splits, along_k, depth, clusters, rounds)
+                mine = -(-chunks // splits)
+                for along_k in (16, 8, 4, 2, 1):
+                    if along_k > warps:
+                        continue
+                    per_unit = warps // along_k
+                    each = -(-mine // along_k)
+                    run = min(2, each)
+                    for depth in (4, 3, 2):
+                        if smem_kb(tokens, warps, splits, 1, depth, run) <= room:
+                            break
+                    else:
+                        continue
+                    at_once = most_clusters(tokens, warps, splits, smem_kb(tokens, warps, splits, 1, depth, run))
+                    if at_once < 1:
+                        continue
+                    units = -(-blocks // per_unit)
+                    clusters = min(units, max(1, at_once // token_blocks))
+                    rounds = -(-units // clusters)
+                    cost = rounds * (per_unit * mine + 2) * (2 if warps == 8 and clusters * splits > 148 else 1) + (20 if splits > 1 else 0)
+                    if best is None or cost < best[0]:
+                        best = (cost, FewRowsPlan(warps, splits, along_k, 1, depth, run, tokens, clusters), rounds, room)
         if best is not None:
-            _, splits, along_k, depth, clusters, rounds = best
+            _, plan, rounds, room = best
             batch = 1
-            while batch < min(rounds, 8) and smem_kb(tokens, splits, batch + 1, depth) <= FEW_SMEM_KB:
+            while batch < min(rounds, 8) and smem_kb(tokens, plan.warps, plan.splits, batch + 1, plan.depth, plan.run) <= room:
                 batch += 1
-            return FewRowsPlan(splits, along_k, batch, depth, tokens, clusters)
+            return plan._replace(batch=batch)
         tokens //= 2
     return None
+
+
+def many_rows_cut(rows: int, columns: int, paired: bool, m: int, sms: int) -> Tuple[int, int]:
+    """(rows of x of a tile, CTAs that share a tile's columns) of the product with many rows of x."""
+    tokens = 32 if m <= 32 else 64 if m <= 64 else 128
+    tiles = -(-rows // (64 if paired else 128)) * -(-m // tokens)
+    chunks = -(-columns // BLOCK_COLS)
+    return tokens, max(1, min(8, sms // tiles, chunks // 2))

@@ -171,6 +171,22 @@ def test_products(kernels, m, n, k, group, x_dtype, out_dtype):
     check_product(kernels, m, n, k, group, x_dtype, out_dtype, residual=out_dtype == F32 and m % 2 == 1)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(17, 128, 128), (32, 257, 1024), (33, 1000, 2056), (64, 40, 4096), (65, 4096, 512), (128, 128, 72), (129, 300, 1000),
+                                   (300, 2051, 1024), (1000, 1024, 2048), (20, 6144, 4096), (2000, 4128, 264), (18, 5, 8)])
+def test_products_with_many_rows(kernels, m, n, k, group, out_dtype):
+    check_product(kernels, m, n, k, group, BF16, out_dtype, residual=out_dtype == F32 and m % 2 == 1)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k,kind", [(17, 64, 128, "silu"), (40, 1000, 512, "gelu_tanh"), (64, 12288, 1024, "silu"), (130, 77, 2000, "silu"),
+                                        (700, 2730, 1024, "gelu_tanh"), (19, 3, 40, "silu")])
+def test_gated_pairs_with_many_rows(kernels, m, n, k, kind, group):
+    check_gated(kernels, m, n, k, group, BF16, kind)
+    check_gated(kernels, m, n, k, group, BF16, kind, out_dtype=F32)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 151936, 256), (1, 128, 32768), (16, 64, 20000), (2, 64, 65536)])
 @pytest.mark.parametrize("x_dtype", [BF16, F32])
 def test_products_of_far_ends(kernels, m, n, k, x_dtype):
@@ -183,9 +199,9 @@ def test_rows_of_x_and_out_with_strides_and_the_residual_in_place(kernels, x_dty
     g = gen(8)
     w = matrix(g, 200, 320, BF16)
     packed, values = kernels.pack_weights(w, 64), packed_values(w, 64)
-    for m in (1, 6, 33):
-        wide = torch.randn(2 * m, 333, generator=g, device=DEV).to(x_dtype)
-        for x in (wide[::2, 1:321], wide[:m, 8:328], wide[:m, :320]):
+    for m in (1, 6, 33, 150):
+        wide = torch.randn(2 * m, 336, generator=g, device=DEV).to(x_dtype)
+        for x in (wide[::2, 1:321], wide[:m, 8:328], wide[:m, :320], wide[:m, 16:].contiguous()):
             room = torch.full((m, 230), 7.0, device=DEV)
             out = room[:, 5:205]
             start = torch.randn(m, 200, generator=g, device=DEV)
@@ -240,8 +256,9 @@ def test_a_group_that_is_no_number_spoils_its_rows_alone(kernels):
     assert out[:, 7].isnan().all() and not out[:, torch.arange(40, device=DEV) != 7].isnan().any()
 
 
-def test_no_rows_and_the_same_bits_twice(kernels):
-    packed, x, out = check_product(kernels, 5, 1000, 2048, 64, BF16, F32)
+@pytest.mark.parametrize("m", [5, 40, 300])
+def test_no_rows_and_the_same_bits_twice(kernels, m):
+    packed, x, out = check_product(kernels, m, 1000, 2048, 64, BF16, F32)
     again = torch.empty_like(out)
     kernels.linear(x, packed, again)
     assert torch.equal(out, again)
@@ -286,13 +303,13 @@ def test_a_gated_pair_with_an_output_of_the_other_type(kernels):
 # ------------------------------------------------------------------ how they are called
 def test_a_captured_product_replays_with_new_rows_of_x(kernels):
     g = gen(20)
-    w = matrix(g, 700, 900, BF16)
+    w = matrix(g, 700, 904, BF16)
     packed, values = kernels.pack_weights(w, 32), packed_values(w, 32)
     pair = kernels.pack_gate_up(w, w.flip(0).contiguous(), 32)
     stream = torch.cuda.Stream()
     graphs = []
-    for m in (1, 11):
-        x = torch.randn(m, 900, generator=g, device=DEV).to(BF16)
+    for m in (1, 11, 50):
+        x = torch.randn(m, 904, generator=g, device=DEV).to(BF16)
         out, gated = torch.empty(m, 700, device=DEV), torch.empty(m, 700, dtype=BF16, device=DEV)
         with torch.cuda.stream(stream):
             kernels.linear(x, packed, out)
