@@ -25,7 +25,7 @@
 namespace chibi {
 namespace {
 
-constexpr int PT_THREADS = 512;                  // loader, issuer, 2 idle warps | 4 converting | 8 adding
+constexpr int PT_THREADS = 640;                  // loader, issuer, 2 idle warps | 8 converting | 8 adding
 constexpr int PT_ROWS = 128;
 constexpr int PT_SCALE_SLOTS = 8;                // blocks of columns whose scales are kept
 
@@ -71,12 +71,52 @@ __device__ __forceinline__ void peer_shared_f32x4(uint32_t own_smem_addr, uint32
                  : "memory");
 }
 
-__device__ __forceinline__ void packed_write(const PackedProduct& p, long long m, int at, float v)
+// An adding warp's columns of a tile: lane l has row l of a record, two neighbouring tokens to a pair.
+template <int COLS, typename OUT>
+__device__ __forceinline__ void write_columns(const PackedProduct& p, const uint64_t (&acc)[COLS / 2], int token0, int left, int n_tile,
+                                              int quarter, int lane)
 {
-    if (p.out_type == CHIBI_F32)
-        static_cast<float*>(p.out)[m * p.out_stride + at] = v;
-    else
-        static_cast<__nv_bfloat16*>(p.out)[m * p.out_stride + at] = from_f32<__nv_bfloat16>(v);
+    OUT* out = static_cast<OUT*>(p.out) + (long long)token0 * p.out_stride;
+    const long long step = p.out_stride;
+    if (p.pair) {
+        // lanes l and l ^ 8 hold a feature's gate and up: one makes the even tokens, the other the odd ones
+        const bool is_up = lane & 8;
+        const int at = n_tile * (PT_ROWS / 2) + quarter * 16 + (lane >> 4) * 8 + (lane & 7);
+        out += at + (is_up ? step : 0);
+        left = at < p.n ? left - (is_up ? 1 : 0) : 0;
+#pragma unroll
+        for (int j = 0; j < COLS / 2; ++j) {
+            const float2 v = halves_of(acc[j]);
+            const float other = __shfl_xor_sync(0xffffffffu, is_up ? v.x : v.y, 8);
+            const float gate = is_up ? other : v.x, up = is_up ? v.y : other;
+            if (2 * j < left)
+                *out = from_f32<OUT>(packed_activate<sizeof(OUT) == 2>(gate, p.act) * up);
+            out += 2 * step;
+        }
+        return;
+    }
+    const int at = n_tile * PT_ROWS + quarter * 32 + lane;
+    if (at >= p.n)
+        return;
+    out += at;
+    const float* residual = p.residual ? p.residual + (long long)token0 * p.residual_stride + at : nullptr;
+#pragma unroll
+    for (int j0 = 0; j0 < COLS; j0 += 8) {
+        float r[8] = {};
+        if (residual) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j0 + j < left)
+                    r[j] = residual[(long long)(j0 + j) * p.residual_stride];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 v = halves_of(acc[(j0 + j) / 2]);
+            if (j0 + j < left)
+                *out = from_f32<OUT>((j & 1 ? v.y : v.x) + r[j]);
+            out += step;
+        }
+    }
 }
 
 template <int TOKENS, int GROUP_BLOCKS>
@@ -105,7 +145,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1 + 4);         // the products have read x, the converting warps the codes
+            mbar_init(&empty[s], 1 + 4);         // the products have read x, four converting warps the codes
         }
         for (int s = 0; s < OPERANDS; ++s) {
             mbar_init(&operand_full[s], 4);
@@ -126,8 +166,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
     tcgen05_fence_after();
     const uint32_t tmem_sums = *tmem_slot, tmem_operands = tmem_sums + SUMS * TOKENS;
 
-    if (warp == 0) {
-        if (elect_one()) {
+    // registers where they are needed: 96 a thread at launch, 5 x 96 = 480 a lane of the five warpgroups
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0 && elect_one()) {
             tma_prefetch_descriptor(&map_x);
             const int per_tile = c1 - c0;
             const long long total = first_tile < p.tiles ? (long long)((p.tiles - 1 - first_tile) / tile_step + 1) * per_tile : 0;
@@ -164,9 +206,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
             // every copy has landed before this CTA's shared memory is anybody else's
             for (long long j = i > STAGES ? i - STAGES : 0; j < i; ++j)
                 mbar_wait(&full[j % STAGES], (uint32_t)(j / STAGES) & 1, p.error, 42);
-        }
-    } else if (warp == 1) {
-        if (elect_one()) {
+        } else if (warp == 1 && elect_one()) {
             constexpr uint32_t idesc = make_idesc_bf16_f32(PT_ROWS, TOKENS);
             constexpr int STEPS = GROUP_BLOCKS * 2;          // 16-column steps of a group
             uint32_t i = 0, a = 0;
@@ -200,14 +240,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                     tcgen05_commit(&empty[s]);
                 }
         }
-    } else if (warp >= 4 && warp < 8) {
-        // ---- codes to bfloat16 in TMEM: a thread its row's 128 columns
+    } else if (warp < 12) {
+        // ---- codes to bfloat16 in TMEM: a thread its row's 128 columns, two warpgroups in turn (one alone is too slow: from the wait to
+        // the last store is a chain of some 1,000 cycles)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const int quarter = warp & 3;
+        const uint32_t turn = (warp - 4) >> 2;
         const uint32_t to = tmem_operands + (static_cast<uint32_t>(quarter * 32) << 16);
         uint32_t i = 0;
         bool ok = true;
         for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step)
             for (int chunk = c0; chunk < c1; ++chunk, ++i) {
+                if ((i & 1) != turn)
+                    continue;
                 const uint32_t s = i % STAGES, o = i % OPERANDS;
                 if (!mbar_wait_warp(&full[s], (i / STAGES) & 1, p.error, 45)) {
                     ok = false;
@@ -254,10 +299,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                 if (lane == 0)
                     mbar_arrive(&operand_full[o]);
             }
-    } else if (warp >= 8) {
+    } else {
         // ---- group sums times scales
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         pdl_wait();
-        const int quarter = warp & 3, half = (warp - 8) >> 2;
+        const int quarter = warp & 3, half = (warp - 12) >> 2;
         const uint32_t from = tmem_sums + (static_cast<uint32_t>(quarter * 32) << 16) + half * COLS;
         constexpr int LOAD = COLS < 32 ? COLS : 32;
         uint32_t i = 0, a = 0;
@@ -311,43 +357,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                 continue;
             }
             const int token0 = tile % p.token_tiles * TOKENS + half * COLS, n_tile = tile / p.token_tiles;
-            if (p.pair) {
-                // lanes l and l ^ 8 hold a feature's gate and up: one makes the even tokens, the other the odd ones
-                const bool is_up = lane & 8;
-                const int at = n_tile * (PT_ROWS / 2) + quarter * 16 + (lane >> 4) * 8 + (lane & 7);
-#pragma unroll
-                for (int j = 0; j < COLS / 2; ++j) {
-                    const float2 v = halves_of(acc[j]);
-                    const float other = __shfl_xor_sync(0xffffffffu, is_up ? v.x : v.y, 8);
-                    const int token = token0 + 2 * j + (is_up ? 1 : 0);
-                    const float gate = is_up ? other : v.x, up = is_up ? v.y : other;
-                    if (token < p.m && at < p.n)
-                        packed_write(p, token, at, (p.out_type == CHIBI_F32 ? activate(gate, p.act) : activate_rounded(gate, p.act)) * up);
-                }
-            } else {
-                const int at = n_tile * PT_ROWS + quarter * 32 + lane;
-                if (at < p.n) {
-#pragma unroll
-                    for (int j0 = 0; j0 < COLS / 2; j0 += 4) {
-                        float r[8] = {};
-                        if (p.residual) {
-#pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                if (token0 + 2 * j0 + j < p.m)
-                                    r[j] = p.residual[(long long)(token0 + 2 * j0 + j) * p.residual_stride + at];
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 v = halves_of(acc[j0 + j]);
-                            const int token = token0 + 2 * (j0 + j);
-                            if (token < p.m)
-                                packed_write(p, token, at, v.x + r[2 * j]);
-                            if (token + 1 < p.m)
-                                packed_write(p, token + 1, at, v.y + r[2 * j + 1]);
-                        }
-                    }
-                }
-            }
+            const int left = p.m - token0;
+            if (p.out_type == CHIBI_F32)
+                write_columns<COLS, float>(p, acc, token0, left, n_tile, quarter, lane);
+            else
+                write_columns<COLS, __nv_bfloat16>(p, acc, token0, left, n_tile, quarter, lane);
         }
     }
 
@@ -385,10 +399,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                 if (at >= p.n)
                     continue;
                 if (p.pair)
-                    v[j] = activate(v[j], p.act) * up[j];
+                    v[j] = (p.out_type == CHIBI_F32 ? packed_activate<false>(v[j], p.act) : packed_activate<true>(v[j], p.act)) * up[j];
                 else if (p.residual)
                     v[j] += p.residual[m * p.residual_stride + at];
-                packed_write(p, m, at, v[j]);
+                if (p.out_type == CHIBI_F32)
+                    static_cast<float*>(p.out)[m * p.out_stride + at] = v[j];
+                else
+                    static_cast<__nv_bfloat16*>(p.out)[m * p.out_stride + at] = from_f32<__nv_bfloat16>(v[j]);
             }
         }
         __syncwarp();

@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows
                 }
             }
             if (p.pair)
-                v = activate(v, p.act) * up;
+                v = (p.out_type == CHIBI_F32 ? packed_activate<false>(v, p.act) : packed_activate<true>(v, p.act)) * up;
             const long long m = token0 + token;
             if (p.residual)
                 v += p.residual[m * p.residual_stride + at];
