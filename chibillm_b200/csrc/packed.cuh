@@ -17,6 +17,7 @@
 // same 8 of up: a lane's two rows of `mma.m16n8k16` are then a feature's gate and its up.
 #pragma once
 #include "common.cuh"
+#include "tensor_map.cuh"
 
 namespace chibi {
 
@@ -38,6 +39,23 @@ __host__ __device__ constexpr int packed_side(int pair, int r) { return pair ? (
 __host__ __device__ constexpr int packed_source_row(int pair, int rb, int r)
 {
     return pair ? rb * (PACKED_ROWS / 2) + (r >> 4) * 8 + (r & 7) : rb * PACKED_ROWS + r;
+}
+
+// A tensor map over the records: a box is `box_cols` neighbouring records of each of `box_rows` blocks of rows, and lands record
+// by record.  (An untiled bulk copy of a record or two is simpler and slower: 17 bytes a cycle and SM.)  A record is two runs of
+// 8-byte elements, since a box has at most 256 in a row.
+inline bool packed_map(const void* data, int group, int row_blocks, int col_blocks, int box_cols, int box_rows, CUtensorMap* out)
+{
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn)
+        return false;
+    const cuuint64_t record = (cuuint64_t)packed_record_bytes(group);
+    const cuuint64_t dims[4] = { record / 16, 2, (cuuint64_t)col_blocks, (cuuint64_t)row_blocks };
+    const cuuint64_t strides[3] = { record / 2, record, record * (cuuint64_t)col_blocks };
+    const cuuint32_t box[4] = { (cuuint32_t)(record / 16), 2, (cuuint32_t)box_cols, (cuuint32_t)box_rows };
+    const cuuint32_t elem[4] = { 1, 1, 1, 1 };
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 4, const_cast<void*>(data), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // The whole numbers of a word as float16, columns 2 j and 2 j + 1 in pair j (exact: 1,024 + code and 1,024 + 16 code have

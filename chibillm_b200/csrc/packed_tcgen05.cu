@@ -49,8 +49,7 @@ template <int TOKENS, int GROUP_BLOCKS> struct PackedTile {
 };
 
 struct PackedProduct {
-    const uint8_t* data;
-    int row_blocks, chunks;                      // blocks of 32 rows, of 128 columns
+    int chunks;                                  // blocks of 128 columns
     int n, pair;
     int m;
     void* out;
@@ -120,7 +119,7 @@ __device__ __forceinline__ void write_columns(const PackedProduct& p, const uint
 }
 
 template <int TOKENS, int GROUP_BLOCKS>
-__global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const __grid_constant__ CUtensorMap map_x, const PackedProduct p)
+__global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const PackedProduct p)
 {
     using namespace sm100;
     using T = PackedTile<TOKENS, GROUP_BLOCKS>;
@@ -170,42 +169,55 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0 && elect_one()) {
+            tma_prefetch_descriptor(&map_w);
             tma_prefetch_descriptor(&map_x);
-            const int per_tile = c1 - c0;
-            const long long total = first_tile < p.tiles ? (long long)((p.tiles - 1 - first_tile) / tile_step + 1) * per_tile : 0;
-            // the codes are constant: those of the first stages are asked for before the kernel ahead has ended
-            auto load_codes = [&](long long i) {
-                const int tile = first_tile + (int)(i / per_tile) * tile_step, chunk = c0 + (int)(i % per_tile);
-                const int s = (int)(i % STAGES), rb = tile / p.token_tiles * (PT_ROWS / PACKED_ROWS);
-                const int records = min(PT_ROWS / PACKED_ROWS, p.row_blocks - rb);
-                mbar_arrive_expect_tx(&full[s], T::X_BYTES + records * RECORD);
-                for (int j = 0; j < records; ++j)
-                    bulk_load(smem + s * T::STAGE + T::X_BYTES + j * RECORD, p.data + ((long long)(rb + j) * p.chunks + chunk) * RECORD,
-                              RECORD, &full[s]);
+            const uint32_t total = first_tile < p.tiles ? ((p.tiles - 1 - first_tile) / tile_step + 1) * (c1 - c0) : 0;
+            // Where the copies of the next block are.  Codes run ahead of x at the start: they are constant, so those of
+            // the first stages are asked for before the kernel ahead has ended.
+            struct Place {
+                int tile, chunk, stage, at;
             };
-            auto load_x = [&](long long i) {
-                const int tile = first_tile + (int)(i / per_tile) * tile_step, chunk = c0 + (int)(i % per_tile);
-                const int s = (int)(i % STAGES), token0 = tile % p.token_tiles * TOKENS;
-                uint8_t* dst = smem + s * T::STAGE;
-                tma_load_2d(dst, &map_x, &full[s], chunk * PACKED_COLS, token0);
-                tma_load_2d(dst + T::X_BYTES / 2, &map_x, &full[s], chunk * PACKED_COLS + 64, token0);
+            Place codes { first_tile - tile_step, c1, 0, 0 }, rows = codes;
+            auto load_codes = [&]() {
+                if (codes.chunk == c1) {
+                    codes.chunk = c0;
+                    codes.tile += tile_step;
+                    codes.at = codes.tile / p.token_tiles * (PT_ROWS / PACKED_ROWS);
+                }
+                mbar_arrive_expect_tx(&full[codes.stage], T::X_BYTES + T::CODE_BYTES);
+                tma_load_4d(smem + codes.stage * T::STAGE + T::X_BYTES, &map_w, &full[codes.stage], 0, 0, codes.chunk, codes.at);
+                ++codes.chunk;
+                codes.stage = codes.stage + 1 == STAGES ? 0 : codes.stage + 1;
             };
-            const int early = total < STAGES ? (int)total : STAGES;
-            for (int i = 0; i < early; ++i)
-                load_codes(i);
+            auto load_x = [&]() {
+                if (rows.chunk == c1) {
+                    rows.chunk = c0;
+                    rows.tile += tile_step;
+                    rows.at = rows.tile % p.token_tiles * TOKENS;
+                }
+                uint8_t* dst = smem + rows.stage * T::STAGE;
+                tma_load_2d(dst, &map_x, &full[rows.stage], rows.chunk * PACKED_COLS, rows.at);
+                tma_load_2d(dst + T::X_BYTES / 2, &map_x, &full[rows.stage], rows.chunk * PACKED_COLS + 64, rows.at);
+                ++rows.chunk;
+                rows.stage = rows.stage + 1 == STAGES ? 0 : rows.stage + 1;
+            };
+            const uint32_t early = min(total, (uint32_t)STAGES);
+            for (uint32_t i = 0; i < early; ++i)
+                load_codes();
             pdl_wait();
-            for (int i = 0; i < early; ++i)
-                load_x(i);
-            long long i = early;
+            for (uint32_t i = 0; i < early; ++i)
+                load_x();
+            uint32_t i = early, round = 0;
             for (; i < total; ++i) {
-                if (!mbar_wait(&empty[i % STAGES], (uint32_t)(i / STAGES - 1) & 1, p.error, 42))
+                if (!mbar_wait(&empty[codes.stage], round & 1, p.error, 42))
                     break;
-                load_codes(i);
-                load_x(i);
+                load_codes();
+                load_x();
+                round += codes.stage == 0;
             }
             // every copy has landed before this CTA's shared memory is anybody else's
-            for (long long j = i > STAGES ? i - STAGES : 0; j < i; ++j)
-                mbar_wait(&full[j % STAGES], (uint32_t)(j / STAGES) & 1, p.error, 42);
+            for (uint32_t j = i > STAGES ? i - STAGES : 0; j < i; ++j)
+                mbar_wait(&full[j % STAGES], (j / STAGES) & 1, p.error, 42);
         } else if (warp == 1 && elect_one()) {
             constexpr uint32_t idesc = make_idesc_bf16_f32(PT_ROWS, TOKENS);
             constexpr int STEPS = GROUP_BLOCKS * 2;          // 16-column steps of a group
@@ -420,7 +432,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
 }
 
 template <int TOKENS, int GROUP_BLOCKS>
-int launch_many_rows(const CUtensorMap& map, const PackedProduct& p, int ctas, cudaStream_t stream)
+int launch_many_rows(const CUtensorMap& map_w, const CUtensorMap& map, const PackedProduct& p, int ctas, cudaStream_t stream)
 {
     constexpr size_t SMEM = PackedTile<TOKENS, GROUP_BLOCKS>::SMEM;
     const cudaError_t e = cudaFuncSetAttribute(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -429,14 +441,15 @@ int launch_many_rows(const CUtensorMap& map, const PackedProduct& p, int ctas, c
         cudaGetLastError();
         return (int)e;
     }
-    launch_cluster_x(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, dim3((unsigned)ctas), dim3(PT_THREADS), SMEM, stream, p.splits, map, p);
+    launch_cluster_x(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, dim3((unsigned)ctas), dim3(PT_THREADS), SMEM, stream, p.splits, map_w, map, p);
     return launch_status();
 }
 
-template <int TOKENS> int launch_many_rows_of(int group, const CUtensorMap& map, const PackedProduct& p, int ctas, cudaStream_t stream)
+template <int TOKENS> int launch_many_rows_of(int group, const CUtensorMap& map_w, const CUtensorMap& map, const PackedProduct& p, int ctas,
+                                              cudaStream_t stream)
 {
-    return group == 32 ? launch_many_rows<TOKENS, 1>(map, p, ctas, stream)
-                       : (group == 64 ? launch_many_rows<TOKENS, 2>(map, p, ctas, stream) : launch_many_rows<TOKENS, 4>(map, p, ctas, stream));
+    return group == 32 ? launch_many_rows<TOKENS, 1>(map_w, map, p, ctas, stream)
+                       : (group == 64 ? launch_many_rows<TOKENS, 2>(map_w, map, p, ctas, stream) : launch_many_rows<TOKENS, 4>(map_w, map, p, ctas, stream));
 }
 
 } // namespace
@@ -462,14 +475,14 @@ CHIBI_API int chibi_packed_many_rows(const void* data, int group, int n, int k, 
     const long long token_tiles = (m + (long long)tokens - 1) / tokens, tiles = (n + (long long)tile_rows - 1) / tile_rows * token_tiles;
     if (tiles * splits > 0x7fffffff)
         return CHIBI_ERR_UNSUPPORTED;
-    CUtensorMap map;
-    if (!tensor_map_2d(x, m, k, x_stride, tokens, &map))
+    CUtensorMap map_w, map;
+    if (!packed_map(data, group, (n + each - 1) / each, chunks, 1, PT_ROWS / PACKED_ROWS, &map_w) || !tensor_map_2d(x, m, k, x_stride, tokens, &map))
         return CHIBI_ERR_UNSUPPORTED;
-    const PackedProduct p { (const uint8_t*)data, (n + each - 1) / each, chunks, n, pair, m, out, out_type, out_stride, (const float*)residual,
+    const PackedProduct p { chunks, n, pair, m, out, out_type, out_stride, (const float*)residual,
                             residual_stride, act, splits, (int)tiles, (int)token_tiles, (int*)error };
     const int sms = device_sm_count();
     const int ctas = splits > 1 ? (int)tiles * splits : (int)(tiles < sms ? tiles : sms);
-    return tokens == 32 ? launch_many_rows_of<32>(group, map, p, ctas, (cudaStream_t)stream)
-                        : (tokens == 64 ? launch_many_rows_of<64>(group, map, p, ctas, (cudaStream_t)stream)
-                                        : launch_many_rows_of<128>(group, map, p, ctas, (cudaStream_t)stream));
+    return tokens == 32 ? launch_many_rows_of<32>(group, map_w, map, p, ctas, (cudaStream_t)stream)
+                        : (tokens == 64 ? launch_many_rows_of<64>(group, map_w, map, p, ctas, (cudaStream_t)stream)
+                                        : launch_many_rows_of<128>(group, map_w, map, p, ctas, (cudaStream_t)stream));
 }

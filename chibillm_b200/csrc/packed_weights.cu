@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(512) unpack_kernel(const uint8_t* data, int ro
 // out[m][n] = sum over groups of s[n][g] * (sum over the group of q[n][k] x[m][k]).
 //
 // What bounds it is the bytes of the matrix.  A CTA of 8 or 16 warps stays on its SM; every warp streams records of its own
-// (bulk copies into a ring of its own, no barrier between warps), makes float16 fragments of the codes and multiplies
+// (tile copies into a ring of its own, no barrier between warps), makes float16 fragments of the codes and multiplies
 // them with x by `mma.m16n8k16`: 16 rows of a record are the instruction's rows, 8 tokens its columns.  x lies in shared
 // memory as the fragments want it, 16 bytes to a lane for four instructions.  Each group's sums start at zero and are
 // multiplied by the scales in 32 bits.
@@ -181,7 +181,6 @@ __global__ void __launch_bounds__(512) unpack_kernel(const uint8_t* data, int ro
 constexpr int FEW_THREADS = 512;             // at most
 
 struct FewRows {
-    const uint8_t* data;
     int row_blocks, chunks;        // blocks of 32 rows, of 128 columns
     int n, k, pair;
     const void* x;
@@ -253,7 +252,7 @@ __device__ __forceinline__ uint32_t take_half_pair(float (&v)[2])
 }
 
 template <int NT, bool X32, int GROUP_BLOCKS>
-__global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows p)
+__global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const __grid_constant__ CUtensorMap map, const FewRows p)
 {
     using namespace sm100;
     using T = typename std::conditional<X32, float, __nv_bfloat16>::type;
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows
 
     // shared memory: rings | x | sums | the rows' largest numbers | barriers
     const uint32_t x_plane = (uint32_t)most * 4 * p.tokens * 64;
-    const int stage = p.run * RECORD;
+    const int stage = (p.run * RECORD + 127) / 128 * 128;        // (a tile copy's place starts on 128 bytes)
     uint8_t* ring = smem + warp * p.depth * stage;
     uint8_t* xs = smem + p.warps * p.depth * stage;
     float* sums = reinterpret_cast<float*>(xs + (size_t)PARTS * x_plane);
@@ -288,21 +287,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows
     const int my_rounds = cluster < units ? (units - 1 - cluster) / p.clusters + 1 : 0;
     const int last_unit = cluster + (my_rounds - 1) * p.clusters;
     const int warp_rounds = my_rounds > 0 && last_unit * blocks_per_unit + wr >= p.row_blocks ? my_rounds - 1 : my_rounds;
-    const long long round_step = ((long long)p.clusters * blocks_per_unit * p.chunks - (w1 - w0)) * RECORD;
-    const uint8_t* next_src = p.data + ((long long)(cluster * blocks_per_unit + wr) * p.chunks + w0) * RECORD;
-    int rounds_to_ask = w1 > w0 ? warp_rounds : 0, next_chunk = w0;
-    // asks for the next records of the warp, up to `run` of one block of rows
+    int rounds_to_ask = w1 > w0 ? warp_rounds : 0, next_chunk = w0, next_block = cluster * blocks_per_unit + wr;
+    // asks for the next `run` records of the warp's block of rows (the last of them may be another warp's, or beyond the matrix)
     auto issue = [&](int slot) {
-        const int bytes = min(p.run, w1 - next_chunk) * RECORD;
         if (lane == 0) {
-            mbar_arrive_expect_tx(&full[slot], bytes);
-            bulk_load(ring + slot * stage, next_src, bytes, &full[slot]);
+            mbar_arrive_expect_tx(&full[slot], p.run * RECORD);
+            tma_load_4d(ring + slot * stage, &map, &full[slot], 0, 0, next_chunk, next_block);
         }
-        next_src += bytes;
         next_chunk += p.run;
         if (next_chunk >= w1) {
             next_chunk = w0;
-            next_src += round_step;
+            next_block += p.clusters * blocks_per_unit;
             --rounds_to_ask;
         }
     };
@@ -535,7 +530,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(FewRows
 }
 
 template <int NT, bool X32>
-void (*few_rows_kernel_of(int group))(FewRows)
+void (*few_rows_kernel_of(int group))(const CUtensorMap, const FewRows)
 {
     return group == 32 ? packed_few_rows_kernel<NT, X32, 1>
                        : (group == 64 ? packed_few_rows_kernel<NT, X32, 2> : packed_few_rows_kernel<NT, X32, 4>);
@@ -546,11 +541,11 @@ constexpr size_t FEW_SMEM_LIMIT = 227 * 1024;
 size_t few_rows_smem(bool x32, int group, int chunks, int warps, int splits, int batch, int depth, int run, int tokens)
 {
     const size_t x_plane = (size_t)((chunks + splits - 1) / splits) * 4 * tokens * 64;
-    return (size_t)warps * depth * run * packed_record_bytes(group) + (x32 ? 2 : 1) * x_plane
+    return (size_t)warps * depth * ((run * packed_record_bytes(group) + 127) / 128 * 128) + (x32 ? 2 : 1) * x_plane
         + (size_t)batch * warps * 256 * (tokens <= 8 ? 1 : 2) * 4 + 16 * 4 + warps * depth * 8;
 }
 
-void (*few_rows_kernel(bool x32, int tokens, int group))(FewRows)
+void (*few_rows_kernel(bool x32, int tokens, int group))(const CUtensorMap, const FewRows)
 {
     return x32 ? (tokens <= 8 ? few_rows_kernel_of<1, true>(group) : few_rows_kernel_of<2, true>(group))
                : (tokens <= 8 ? few_rows_kernel_of<1, false>(group) : few_rows_kernel_of<2, false>(group));
@@ -619,7 +614,7 @@ CHIBI_API int chibi_packed_few_rows_clusters(int x32, int group, int tokens, int
 {
     if (!packed_group_ok(group) || splits < 1 || splits > 8 || tokens < 1 || tokens > 16 || kb < 1 || kb > 227 || warps < 1 || warps > 16)
         return 0;
-    void (*kernel)(FewRows) = few_rows_kernel(x32 != 0, tokens, group);
+    void (*kernel)(const CUtensorMap, const FewRows) = few_rows_kernel(x32 != 0, tokens, group);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)splits);
     cfg.blockDim = dim3((unsigned)warps * 32);
@@ -658,15 +653,18 @@ CHIBI_API int chibi_packed_few_rows(const void* data, int group, int n, int k, i
     const int each = pair ? PACKED_ROWS / 2 : PACKED_ROWS;
     if (smem > FEW_SMEM_LIMIT || token_blocks > 65535)
         return CHIBI_ERR_UNSUPPORTED;
-    const FewRows p { (const uint8_t*)data, (n + each - 1) / each, chunks, n, k, pair, x, x_stride, m, out, out_type, out_stride,
+    CUtensorMap map;
+    if (run > 256 || !packed_map(data, group, (n + each - 1) / each, chunks, run, 1, &map))
+        return CHIBI_ERR_UNSUPPORTED;
+    const FewRows p { (n + each - 1) / each, chunks, n, k, pair, x, x_stride, m, out, out_type, out_stride,
                       (const float*)residual, residual_stride, act, warps, splits, along_k, batch, depth, run, tokens, clusters, (int*)error };
-    void (*kernel)(FewRows) = few_rows_kernel(x32, tokens, group);
+    void (*kernel)(const CUtensorMap, const FewRows) = few_rows_kernel(x32, tokens, group);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SMEM_LIMIT);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return (int)e;
     }
     launch_cluster_x(kernel, dim3((unsigned)(clusters * splits), (unsigned)token_blocks), dim3((unsigned)warps * 32), smem,
-                     (cudaStream_t)stream, splits, p);
+                     (cudaStream_t)stream, splits, map, p);
     return launch_status();
 }
