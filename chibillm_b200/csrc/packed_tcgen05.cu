@@ -4,14 +4,13 @@
 //
 // The matrix's 128 rows of a tile are the instruction's rows, TOKENS rows of x its columns.  Warps that do nothing else turn
 // codes into bfloat16 whole numbers (exact) and write them to TMEM, where they are the A operand: shared memory carries only
-// the rows of x and the codes themselves.  Each group's sum is an accumulator of its own in TMEM; two warpgroups read it, each
-// half of the columns, and add it times the row's scale to sums in registers.  So nothing is rounded but 32-bit sums, and a
+// the rows of x and the codes themselves.  Each group's sum is an accumulator of its own in TMEM; three warpgroups read it, each
+// a third of the columns, and add it times the row's scale to sums in registers.  So nothing is rounded but 32-bit sums, and a
 // lane's row has one scale for all of its columns.  A thread's sums are an output column of 32 lanes: stores are whole
 // lines without a detour.
 //
-// What bounds it: with 128 tokens a tile, a block of 128 columns takes the tensor cores 512 cycles (8,192 multiply-adds
-// a cycle and SM for 128 x 128 x 128), the four converting warps some 250 instructions each, the eight adding warps 64 columns for each
-// group; at groups of 32 reading TMEM (four times as often as at 128) takes as long as the products.
+// What bounds it: an instruction of 128 x TOKENS x 16 with its A operand in TMEM takes 118 cycles at 64 as at 128 columns, so tiles
+// are 192 tokens wide, the most that leaves room in TMEM for two accumulators and two operands (two of 192 columns, two of 64).
 //
 // Few tiles: `splits` CTAs of a cluster share a tile's columns; their sums go to shared memory and each CTA adds up a
 // share of them, CTA by CTA in one order.
@@ -25,27 +24,28 @@
 namespace chibi {
 namespace {
 
-constexpr int PT_THREADS = 640;                  // loader, issuer, 2 idle warps | 8 converting | 8 adding
+constexpr int PT_ADDERS = 12;                    // warps
+constexpr int PT_THREADS = (4 + 4 + PT_ADDERS) * 32;             // codes' loader, issuer, x's loader, an idle warp | converting | adding
 constexpr int PT_ROWS = 128;
 constexpr int PT_SCALE_SLOTS = 8;                // blocks of columns whose scales are kept
 
 template <int TOKENS, int GROUP_BLOCKS> struct PackedTile {
     static constexpr int GROUPS = 4 / GROUP_BLOCKS;
     static constexpr int RECORD = PACKED_CODE_BYTES + GROUPS * 64;
-    static constexpr int X_BYTES = TOKENS * PACKED_COLS * 2, CODE_BYTES = PT_ROWS / PACKED_ROWS * RECORD;
-    static constexpr int CODE_ROOM = (CODE_BYTES + 1023) / 1024 * 1024;
-    static constexpr int STAGE = X_BYTES + CODE_ROOM;
+    static constexpr int X_BYTES = TOKENS * PACKED_COLS * 2, X_STAGES = TOKENS > 96 ? 3 : TOKENS > 48 ? 4 : 6;
+    static constexpr int CODE_BYTES = PT_ROWS / PACKED_ROWS * RECORD, CODE_STAGES = TOKENS > 96 ? 4 : 6;
+    static_assert(CODE_BYTES % 128 == 0 && X_BYTES % 2048 == 0, "a tile copy's place");
     static constexpr int SCALES = PT_SCALE_SLOTS * GROUPS * PT_ROWS * 4;
-    static constexpr int BUDGET = 226 * 1024 - 1024 - SCALES - 1024;
-    static constexpr int STAGES = BUDGET / STAGE > 6 ? 6 : BUDGET / STAGE;
     // accumulators (one for each group on its way) and operand blocks in TMEM's 512 columns
-    static constexpr int SUMS = TOKENS <= 64 ? 4 : 2, OPERANDS = (512 - SUMS * TOKENS) / 64 > 4 ? 4 : (512 - SUMS * TOKENS) / 64;
-    static constexpr size_t SMEM = 1024 + STAGES * STAGE + SCALES + (2 * STAGES + 2 * OPERANDS + 2 * SUMS) * 8 + 16;
-    static_assert(STAGES >= 2 && OPERANDS >= 2, "");
+    static constexpr int SUMS = TOKENS > 96 ? 2 : TOKENS > 48 ? 3 : 4, OPERANDS = SUMS;
+    static_assert(SUMS * TOKENS + OPERANDS * 64 <= 512, "");
     // Block i's scales go where block i - 8's were.  Its operand's place is free when the products of block i - OPERANDS are
     // done, which began when all groups but the last SUMS up to there had been added up: those of block i - 8 among them.
     static_assert(SUMS <= (PT_SCALE_SLOTS - OPERANDS) * GROUPS, "");
-    static_assert(STAGES * STAGE >= TOKENS * PT_ROWS * 4, "a tile's sums fit where the stages were");
+    static constexpr size_t SMEM = 1024 + X_STAGES * X_BYTES + CODE_STAGES * CODE_BYTES + SCALES
+        + 2 * (X_STAGES + CODE_STAGES + OPERANDS + SUMS) * 8 + 16;
+    static_assert(X_STAGES * X_BYTES >= TOKENS * PT_ROWS * 4, "a tile's sums fit where x was");
+    static_assert(SMEM <= 227 * 1024, "");
 };
 
 struct PackedProduct {
@@ -123,15 +123,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
 {
     using namespace sm100;
     using T = PackedTile<TOKENS, GROUP_BLOCKS>;
-    constexpr int GROUPS = T::GROUPS, RECORD = T::RECORD, STAGES = T::STAGES, OPERANDS = T::OPERANDS, SUMS = T::SUMS;
-    constexpr int COLS = TOKENS / 2;             // of an adding warpgroup
+    constexpr int GROUPS = T::GROUPS, RECORD = T::RECORD, X_STAGES = T::X_STAGES, CODE_STAGES = T::CODE_STAGES;
+    constexpr int OPERANDS = T::OPERANDS, SUMS = T::SUMS;
+    constexpr int COLS = TOKENS / (PT_ADDERS / 4);           // of an adding warpgroup
     pdl_trigger();
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* scales = reinterpret_cast<float*>(smem + STAGES * T::STAGE);          // [slot][group][row]
-    uint64_t* full = reinterpret_cast<uint64_t*>(scales + T::SCALES / 4);         // a stage's codes and rows of x are there
-    uint64_t* empty = full + STAGES;
-    uint64_t* operand_full = empty + STAGES;
+    uint8_t* xs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* codes = xs + X_STAGES * T::X_BYTES;
+    float* scales = reinterpret_cast<float*>(codes + CODE_STAGES * T::CODE_BYTES);        // [slot][group][row]
+    uint64_t* x_full = reinterpret_cast<uint64_t*>(scales + T::SCALES / 4);
+    uint64_t* x_empty = x_full + X_STAGES;
+    uint64_t* codes_full = x_empty + X_STAGES;
+    uint64_t* codes_empty = codes_full + CODE_STAGES;
+    uint64_t* operand_full = codes_empty + CODE_STAGES;
     uint64_t* operand_empty = operand_full + OPERANDS;
     uint64_t* sums_full = operand_empty + OPERANDS;
     uint64_t* sums_empty = sums_full + SUMS;
@@ -142,9 +146,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
     const int first_tile = blockIdx.x / p.splits, tile_step = gridDim.x / p.splits;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1 + 4);         // the products have read x, four converting warps the codes
+        for (int s = 0; s < X_STAGES; ++s) {
+            mbar_init(&x_full[s], 1);
+            mbar_init(&x_empty[s], 1);
+        }
+        for (int s = 0; s < CODE_STAGES; ++s) {
+            mbar_init(&codes_full[s], 1);
+            mbar_init(&codes_empty[s], 4);
         }
         for (int s = 0; s < OPERANDS; ++s) {
             mbar_init(&operand_full[s], 4);
@@ -152,7 +160,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
         }
         for (int s = 0; s < SUMS; ++s) {
             mbar_init(&sums_full[s], 1);
-            mbar_init(&sums_empty[s], 8);
+            mbar_init(&sums_empty[s], PT_ADDERS);
         }
         fence_barrier_init();
     }
@@ -165,59 +173,51 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
     tcgen05_fence_after();
     const uint32_t tmem_sums = *tmem_slot, tmem_operands = tmem_sums + SUMS * TOKENS;
 
-    // registers where they are needed: 96 a thread at launch, 5 x 96 = 480 a lane of the five warpgroups
+    // registers where they are needed: 96 a thread at launch, 5 x 96 = 480 >= 40 + 88 + 3 x 112 a lane of the five warpgroups
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0 && elect_one()) {
+            // ---- codes: constant, so they are asked for before the kernel ahead has ended
             tma_prefetch_descriptor(&map_w);
-            tma_prefetch_descriptor(&map_x);
-            const uint32_t total = first_tile < p.tiles ? ((p.tiles - 1 - first_tile) / tile_step + 1) * (c1 - c0) : 0;
-            // Where the copies of the next block are.  Codes run ahead of x at the start: they are constant, so those of
-            // the first stages are asked for before the kernel ahead has ended.
-            struct Place {
-                int tile, chunk, stage, at;
-            };
-            Place codes { first_tile - tile_step, c1, 0, 0 }, rows = codes;
-            auto load_codes = [&]() {
-                if (codes.chunk == c1) {
-                    codes.chunk = c0;
-                    codes.tile += tile_step;
-                    codes.at = codes.tile / p.token_tiles * (PT_ROWS / PACKED_ROWS);
+            uint32_t i = 0, s = 0;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step) {
+                const int rb = tile / p.token_tiles * (PT_ROWS / PACKED_ROWS);
+                for (int chunk = c0; chunk < c1; ++chunk, ++i) {
+                    if (i >= CODE_STAGES && !mbar_wait(&codes_empty[s], (i / CODE_STAGES - 1) & 1, p.error, 42)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_expect_tx(&codes_full[s], T::CODE_BYTES);
+                    tma_load_4d(codes + s * T::CODE_BYTES, &map_w, &codes_full[s], 0, 0, chunk, rb);
+                    s = s + 1 == CODE_STAGES ? 0 : s + 1;
                 }
-                mbar_arrive_expect_tx(&full[codes.stage], T::X_BYTES + T::CODE_BYTES);
-                tma_load_4d(smem + codes.stage * T::STAGE + T::X_BYTES, &map_w, &full[codes.stage], 0, 0, codes.chunk, codes.at);
-                ++codes.chunk;
-                codes.stage = codes.stage + 1 == STAGES ? 0 : codes.stage + 1;
-            };
-            auto load_x = [&]() {
-                if (rows.chunk == c1) {
-                    rows.chunk = c0;
-                    rows.tile += tile_step;
-                    rows.at = rows.tile % p.token_tiles * TOKENS;
-                }
-                uint8_t* dst = smem + rows.stage * T::STAGE;
-                tma_load_2d(dst, &map_x, &full[rows.stage], rows.chunk * PACKED_COLS, rows.at);
-                tma_load_2d(dst + T::X_BYTES / 2, &map_x, &full[rows.stage], rows.chunk * PACKED_COLS + 64, rows.at);
-                ++rows.chunk;
-                rows.stage = rows.stage + 1 == STAGES ? 0 : rows.stage + 1;
-            };
-            const uint32_t early = min(total, (uint32_t)STAGES);
-            for (uint32_t i = 0; i < early; ++i)
-                load_codes();
-            pdl_wait();
-            for (uint32_t i = 0; i < early; ++i)
-                load_x();
-            uint32_t i = early, round = 0;
-            for (; i < total; ++i) {
-                if (!mbar_wait(&empty[codes.stage], round & 1, p.error, 42))
-                    break;
-                load_codes();
-                load_x();
-                round += codes.stage == 0;
             }
             // every copy has landed before this CTA's shared memory is anybody else's
-            for (uint32_t j = i > STAGES ? i - STAGES : 0; j < i; ++j)
-                mbar_wait(&full[j % STAGES], (j / STAGES) & 1, p.error, 42);
+            for (uint32_t j = i > CODE_STAGES ? i - CODE_STAGES : 0; j < i; ++j)
+                mbar_wait(&codes_full[j % CODE_STAGES], (j / CODE_STAGES) & 1, p.error, 42);
+        } else if (warp == 2 && elect_one()) {
+            // ---- rows of x
+            tma_prefetch_descriptor(&map_x);
+            pdl_wait();
+            uint32_t i = 0, s = 0;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step) {
+                const int token0 = tile % p.token_tiles * TOKENS;
+                for (int chunk = c0; chunk < c1; ++chunk, ++i) {
+                    if (i >= X_STAGES && !mbar_wait(&x_empty[s], (i / X_STAGES - 1) & 1, p.error, 42)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* dst = xs + s * T::X_BYTES;
+                    mbar_arrive_expect_tx(&x_full[s], T::X_BYTES);
+                    tma_load_2d(dst, &map_x, &x_full[s], chunk * PACKED_COLS, token0);
+                    tma_load_2d(dst + T::X_BYTES / 2, &map_x, &x_full[s], chunk * PACKED_COLS + 64, token0);
+                    s = s + 1 == X_STAGES ? 0 : s + 1;
+                }
+            }
+            for (uint32_t j = i > X_STAGES ? i - X_STAGES : 0; j < i; ++j)
+                mbar_wait(&x_full[j % X_STAGES], (j / X_STAGES) & 1, p.error, 42);
         } else if (warp == 1 && elect_one()) {
             constexpr uint32_t idesc = make_idesc_bf16_f32(PT_ROWS, TOKENS);
             constexpr int STEPS = GROUP_BLOCKS * 2;          // 16-column steps of a group
@@ -225,12 +225,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
             bool ok = true;
             for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step)
                 for (int chunk = c0; ok && chunk < c1; ++chunk, ++i) {
-                    const uint32_t s = i % STAGES, o = i % OPERANDS;
-                    if (!mbar_wait(&full[s], (i / STAGES) & 1, p.error, 43) || !mbar_wait(&operand_full[o], (i / OPERANDS) & 1, p.error, 43)) {
+                    const uint32_t s = i % X_STAGES, o = i % OPERANDS;
+                    if (!mbar_wait(&x_full[s], (i / X_STAGES) & 1, p.error, 43) || !mbar_wait(&operand_full[o], (i / OPERANDS) & 1, p.error, 43)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t x_addr = smem_addr(smem + s * T::STAGE);
+                    const uint64_t x_desc = make_kmajor_sw128_desc(smem_addr(xs + s * T::X_BYTES));
 #pragma unroll
                     for (int g = 0; g < GROUPS; ++g, ++a) {
                         const uint32_t d = a % SUMS;
@@ -242,35 +242,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
 #pragma unroll
                         for (int k = 0; k < STEPS; ++k) {
                             const int step = g * STEPS + k;
+                            // (the address field counts 16 bytes)
                             tcgen05_mma_bf16_a_tmem(tmem_sums + d * TOKENS, tmem_operands + o * 64 + step * 8,
-                                                    make_kmajor_sw128_desc(x_addr + (step >> 2) * (T::X_BYTES / 2) + (step & 3) * 32), idesc,
-                                                    k > 0 ? 1u : 0u);
+                                                    x_desc + ((step >> 2) * (T::X_BYTES / 2) + (step & 3) * 32) / 16, idesc, k > 0 ? 1u : 0u);
                         }
                         tcgen05_commit(&sums_full[d]);
                     }
                     tcgen05_commit(&operand_empty[o]);
-                    tcgen05_commit(&empty[s]);
+                    tcgen05_commit(&x_empty[s]);
                 }
         }
-    } else if (warp < 12) {
-        // ---- codes to bfloat16 in TMEM: a thread its row's 128 columns, two warpgroups in turn (one alone is too slow: from the wait to
-        // the last store is a chain of some 1,000 cycles)
+    } else if (warp < 8) {
+        // ---- codes to bfloat16 in TMEM: a thread its row's 128 columns
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const int quarter = warp & 3;
-        const uint32_t turn = (warp - 4) >> 2;
         const uint32_t to = tmem_operands + (static_cast<uint32_t>(quarter * 32) << 16);
         uint32_t i = 0;
         bool ok = true;
         for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step)
             for (int chunk = c0; chunk < c1; ++chunk, ++i) {
-                if ((i & 1) != turn)
-                    continue;
-                const uint32_t s = i % STAGES, o = i % OPERANDS;
-                if (!mbar_wait_warp(&full[s], (i / STAGES) & 1, p.error, 45)) {
+                const uint32_t s = i % CODE_STAGES, o = i % OPERANDS;
+                if (!mbar_wait_warp(&codes_full[s], (i / CODE_STAGES) & 1, p.error, 45)) {
                     ok = false;
                     break;
                 }
-                const uint8_t* rec = smem + s * T::STAGE + T::X_BYTES + quarter * RECORD;
+                const uint8_t* rec = codes + s * T::CODE_BYTES + quarter * RECORD;
                 uint32_t w[4][4];                // [piece][word]
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
@@ -281,18 +277,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                     sc[g] = to_f32(*reinterpret_cast<const __nv_bfloat16*>(rec + packed_scale_at(lane, g)));
                 __syncwarp();
                 if (lane == 0)
-                    mbar_arrive(&empty[s]);
-                if (i >= OPERANDS && !mbar_wait_warp(&operand_empty[o], (i / OPERANDS - 1) & 1, p.error, 46)) {
-                    ok = false;
-                    break;
-                }
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g)
-                    scales[((i % PT_SCALE_SLOTS) * GROUPS + g) * PT_ROWS + quarter * 32 + lane] = sc[g];
-                tcgen05_fence_after();
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t v[32];
+                    mbar_arrive(&codes_empty[s]);
+                uint32_t v[32];
+                auto convert = [&](int half) {
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -303,8 +290,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                             v[b * 16 + c * 4 + 2] = packed_bf16_pair<2>(word);
                             v[b * 16 + c * 4 + 3] = packed_bf16_pair<3>(word);
                         }
-                    tmem_store_32x32(to + o * 64 + half * 32, v);
+                };
+                // (the first half while the products before still read the operand's place)
+                convert(0);
+                if (i >= OPERANDS && !mbar_wait_warp(&operand_empty[o], (i / OPERANDS - 1) & 1, p.error, 46)) {
+                    ok = false;
+                    break;
                 }
+                tcgen05_fence_after();
+                tmem_store_32x32(to + o * 64, v);
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g)
+                    scales[((i % PT_SCALE_SLOTS) * GROUPS + g) * PT_ROWS + quarter * 32 + lane] = sc[g];
+                convert(1);
+                tmem_store_32x32(to + o * 64 + 32, v);
                 tmem_store_wait();
                 tcgen05_fence_before();
                 __syncwarp();
@@ -313,10 +312,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
             }
     } else {
         // ---- group sums times scales
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
         pdl_wait();
-        const int quarter = warp & 3, half = (warp - 12) >> 2;
-        const uint32_t from = tmem_sums + (static_cast<uint32_t>(quarter * 32) << 16) + half * COLS;
+        const int quarter = warp & 3, part = (warp - 8) >> 2;
+        const uint32_t from = tmem_sums + (static_cast<uint32_t>(quarter * 32) << 16) + part * COLS;
         constexpr int LOAD = COLS < 32 ? COLS : 32;
         uint32_t i = 0, a = 0;
         bool ok = true;
@@ -358,8 +357,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
             if (!ok)
                 break;
             if (p.splits > 1) {
-                // [column][row], where the stages were: all of this tile's copies and products are done, and there is one tile
-                float* mine = reinterpret_cast<float*>(smem) + half * COLS * PT_ROWS + quarter * 32 + lane;
+                // [column][row], where x was: all of this tile's copies and products are done, and there is one tile
+                float* mine = reinterpret_cast<float*>(xs) + part * COLS * PT_ROWS + quarter * 32 + lane;
 #pragma unroll
                 for (int j = 0; j < COLS / 2; ++j) {
                     const float2 v = halves_of(acc[j]);
@@ -368,7 +367,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                 }
                 continue;
             }
-            const int token0 = tile % p.token_tiles * TOKENS + half * COLS, n_tile = tile / p.token_tiles;
+            const int token0 = tile % p.token_tiles * TOKENS + part * COLS, n_tile = tile / p.token_tiles;
             const int left = p.m - token0;
             if (p.out_type == CHIBI_F32)
                 write_columns<COLS, float>(p, acc, token0, left, n_tile, quarter, lane);
@@ -386,7 +385,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
         const int token0 = first_tile % p.token_tiles * TOKENS, n_tile = first_tile / p.token_tiles;
         const int tokens = min(TOKENS, p.m - token0);
         const int t0 = tokens * rank / p.splits, t1 = tokens * (rank + 1) / p.splits;
-        const uint32_t base = smem_addr(smem);
+        const uint32_t base = smem_addr(xs);
         for (int e = threadIdx.x; e < (t1 - t0) * (PT_ROWS / 4); e += PT_THREADS) {
             const int token = t0 + e / (PT_ROWS / 4), row = e % (PT_ROWS / 4) * 4;
             const bool up_rows = p.pair && (row & 8);
@@ -467,7 +466,7 @@ CHIBI_API int chibi_packed_many_rows(const void* data, int group, int n, int k, 
         || (pair && (residual || (act != 1 && act != 2))))
         return CHIBI_ERR_ARGUMENT;
     const int chunks = (k + PACKED_COLS - 1) / PACKED_COLS;
-    if ((tokens != 32 && tokens != 64 && tokens != 128) || splits < 1 || splits > 8 || splits > chunks)
+    if ((tokens != 48 && tokens != 96 && tokens != 192) || splits < 1 || splits > 8 || splits > chunks)
         return CHIBI_ERR_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(x) & 15) || x_stride % 8)
         return CHIBI_ERR_UNSUPPORTED;
@@ -482,7 +481,7 @@ CHIBI_API int chibi_packed_many_rows(const void* data, int group, int n, int k, 
                             residual_stride, act, splits, (int)tiles, (int)token_tiles, (int*)error };
     const int sms = device_sm_count();
     const int ctas = splits > 1 ? (int)tiles * splits : (int)(tiles < sms ? tiles : sms);
-    return tokens == 32 ? launch_many_rows_of<32>(group, map_w, map, p, ctas, (cudaStream_t)stream)
-                        : (tokens == 64 ? launch_many_rows_of<64>(group, map_w, map, p, ctas, (cudaStream_t)stream)
-                                        : launch_many_rows_of<128>(group, map_w, map, p, ctas, (cudaStream_t)stream));
+    return tokens == 48 ? launch_many_rows_of<48>(group, map_w, map, p, ctas, (cudaStream_t)stream)
+                        : (tokens == 96 ? launch_many_rows_of<96>(group, map_w, map, p, ctas, (cudaStream_t)stream)
+                                        : launch_many_rows_of<192>(group, map_w, map, p, ctas, (cudaStream_t)stream));
 }

@@ -102,7 +102,7 @@ def few_rows_plan(rows: int, columns: int, paired: bool, m: int, smem_kb: Callab
 
 def many_rows_cut(rows: int, columns: int, paired: bool, m: int, sms: int) -> Tuple[int, int]:
     """(rows of x of a tile, CTAs that share a tile's columns) of the product with many rows of x."""
-    tokens = 32 if m <= 32 else 64 if m <= 64 else 128
+    tokens = 48 if m <= 48 else 96 if m <= 96 else 192
     tiles = -(-rows // (64 if paired else 128)) * -(-m // tokens)
     chunks = -(-columns // BLOCK_COLS)
     return tokens, max(1, min(8, sms // tiles, chunks // 2))

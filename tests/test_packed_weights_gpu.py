@@ -174,7 +174,8 @@ def test_products(kernels, m, n, k, group, x_dtype, out_dtype):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("out_dtype", [BF16, F32])
 @pytest.mark.parametrize("m,n,k", [(17, 128, 128), (32, 257, 1024), (33, 1000, 2056), (64, 40, 4096), (65, 4096, 512), (128, 128, 72), (129, 300, 1000),
-                                   (300, 2051, 1024), (1000, 1024, 2048), (20, 6144, 4096), (2000, 4128, 264), (18, 5, 8)])
+                                   (300, 2051, 1024), (1000, 1024, 2048), (20, 6144, 4096), (2000, 4128, 264), (18, 5, 8),
+                                   (48, 1000, 640), (49, 1000, 640), (96, 200, 1664), (97, 200, 1664), (192, 4096, 384), (193, 4096, 384)])
 def test_products_with_many_rows(kernels, m, n, k, group, out_dtype):
     check_product(kernels, m, n, k, group, BF16, out_dtype, residual=out_dtype == F32 and m % 2 == 1)
 
