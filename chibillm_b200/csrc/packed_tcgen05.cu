@@ -12,8 +12,9 @@
 // What bounds it: an instruction of 128 x TOKENS x 16 with its A operand in TMEM takes 118 cycles at 64 as at 128 columns, so tiles
 // are 192 tokens wide, the most that leaves room in TMEM for two accumulators and two operands (two of 192 columns, two of 64).
 //
-// Few tiles: `splits` CTAs of a cluster share a tile's columns; their sums go to shared memory and each CTA adds up a
-// share of them, CTA by CTA in one order.
+// A CTA stays on its SM and takes tiles in turn.  What is left after whole rounds of tiles (all of them, if they are few) is shared
+// out: `splits` CTAs of a cluster share a tile's columns; their sums go to shared memory and each CTA adds up a share of them,
+// CTA by CTA in one order.
 #define CHIBI_UNIT packed_tcgen05
 #define CHIBI_UNIT_ID 20
 #include "packed.cuh"
@@ -58,7 +59,7 @@ struct PackedProduct {
     const float* residual;
     long long residual_stride;
     int act;                                     // pairs: 1 gelu with tanh, 2 silu
-    int splits, tiles, token_tiles;
+    int rounds, splits, tiles, token_tiles;      // see piece()
     int* error;
 };
 
@@ -142,8 +143,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_empty + SUMS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = p.splits > 1 ? (int)cluster_cta_rank() : 0;
-    const int c0 = (int)((long long)p.chunks * rank / p.splits), c1 = (int)((long long)p.chunks * (rank + 1) / p.splits);
-    const int first_tile = blockIdx.x / p.splits, tile_step = gridDim.x / p.splits;
+    // A CTA's r-th piece of work, blocks c0 ... c1 of a tile: `rounds` whole tiles, then, in clusters, its share of one more.
+    struct Piece {
+        int tile, c0, c1;
+    };
+    auto piece = [&](int r, Piece& out) -> bool {
+        out = { (int)(blockIdx.x + r * gridDim.x), 0, p.chunks };
+        if (r == p.rounds)
+            out = { (int)(p.rounds * gridDim.x + blockIdx.x / p.splits), p.chunks * rank / p.splits, p.chunks * (rank + 1) / p.splits };
+        return out.tile < p.tiles && (r < p.rounds || (r == p.rounds && p.splits > 1));
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < X_STAGES; ++s) {
@@ -181,9 +190,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
             tma_prefetch_descriptor(&map_w);
             uint32_t i = 0, s = 0;
             bool ok = true;
-            for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step) {
-                const int rb = tile / p.token_tiles * (PT_ROWS / PACKED_ROWS);
-                for (int chunk = c0; chunk < c1; ++chunk, ++i) {
+            Piece at;
+            for (int r = 0; ok && piece(r, at); ++r) {
+                const int rb = at.tile / p.token_tiles * (PT_ROWS / PACKED_ROWS);
+                for (int chunk = at.c0; chunk < at.c1; ++chunk, ++i) {
                     if (i >= CODE_STAGES && !mbar_wait(&codes_empty[s], (i / CODE_STAGES - 1) & 1, p.error, 42)) {
                         ok = false;
                         break;
@@ -202,9 +212,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
             pdl_wait();
             uint32_t i = 0, s = 0;
             bool ok = true;
-            for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step) {
-                const int token0 = tile % p.token_tiles * TOKENS;
-                for (int chunk = c0; chunk < c1; ++chunk, ++i) {
+            Piece at;
+            for (int r = 0; ok && piece(r, at); ++r) {
+                const int token0 = at.tile % p.token_tiles * TOKENS;
+                for (int chunk = at.c0; chunk < at.c1; ++chunk, ++i) {
                     if (i >= X_STAGES && !mbar_wait(&x_empty[s], (i / X_STAGES - 1) & 1, p.error, 42)) {
                         ok = false;
                         break;
@@ -223,8 +234,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
             constexpr int STEPS = GROUP_BLOCKS * 2;          // 16-column steps of a group
             uint32_t i = 0, a = 0;
             bool ok = true;
-            for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step)
-                for (int chunk = c0; ok && chunk < c1; ++chunk, ++i) {
+            Piece at;
+            for (int r = 0; ok && piece(r, at); ++r)
+                for (int chunk = at.c0; ok && chunk < at.c1; ++chunk, ++i) {
                     const uint32_t s = i % X_STAGES, o = i % OPERANDS;
                     if (!mbar_wait(&x_full[s], (i / X_STAGES) & 1, p.error, 43) || !mbar_wait(&operand_full[o], (i / OPERANDS) & 1, p.error, 43)) {
                         ok = false;
@@ -259,8 +271,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
         const uint32_t to = tmem_operands + (static_cast<uint32_t>(quarter * 32) << 16);
         uint32_t i = 0;
         bool ok = true;
-        for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step)
-            for (int chunk = c0; chunk < c1; ++chunk, ++i) {
+        Piece at;
+        for (int r = 0; ok && piece(r, at); ++r)
+            for (int chunk = at.c0; chunk < at.c1; ++chunk, ++i) {
                 const uint32_t s = i % CODE_STAGES, o = i % OPERANDS;
                 if (!mbar_wait_warp(&codes_full[s], (i / CODE_STAGES) & 1, p.error, 45)) {
                     ok = false;
@@ -319,12 +332,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
         constexpr int LOAD = COLS < 32 ? COLS : 32;
         uint32_t i = 0, a = 0;
         bool ok = true;
-        for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step) {
+        Piece at;
+        for (int r = 0; ok && piece(r, at); ++r) {
             uint64_t acc[COLS / 2];
 #pragma unroll
             for (int j = 0; j < COLS / 2; ++j)
                 acc[j] = 0;
-            for (int chunk = c0; ok && chunk < c1; ++chunk, ++i)
+            for (int chunk = at.c0; ok && chunk < at.c1; ++chunk, ++i)
 #pragma unroll 1
                 for (int g = 0; g < GROUPS; ++g, ++a) {
                     const uint32_t d = a % SUMS;
@@ -356,8 +370,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                 }
             if (!ok)
                 break;
-            if (p.splits > 1) {
-                // [column][row], where x was: all of this tile's copies and products are done, and there is one tile
+            if (r == p.rounds) {
+                // [column][row], where x was: all of this CTA's copies and products are done
                 float* mine = reinterpret_cast<float*>(xs) + part * COLS * PT_ROWS + quarter * 32 + lane;
 #pragma unroll
                 for (int j = 0; j < COLS / 2; ++j) {
@@ -367,7 +381,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                 }
                 continue;
             }
-            const int token0 = tile % p.token_tiles * TOKENS + part * COLS, n_tile = tile / p.token_tiles;
+            const int token0 = at.tile % p.token_tiles * TOKENS + part * COLS, n_tile = at.tile / p.token_tiles;
             const int left = p.m - token0;
             if (p.out_type == CHIBI_F32)
                 write_columns<COLS, float>(p, acc, token0, left, n_tile, quarter, lane);
@@ -382,8 +396,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
         __syncthreads();
         cluster_sync();
         // every CTA of the cluster adds up a share of the tile's columns, four rows a thread
-        const int token0 = first_tile % p.token_tiles * TOKENS, n_tile = first_tile / p.token_tiles;
-        const int tokens = min(TOKENS, p.m - token0);
+        Piece at;
+        const bool any = piece(p.rounds, at);
+        const int token0 = at.tile % p.token_tiles * TOKENS, n_tile = at.tile / p.token_tiles;
+        const int tokens = any ? min(TOKENS, p.m - token0) : 0;
         const int t0 = tokens * rank / p.splits, t1 = tokens * (rank + 1) / p.splits;
         const uint32_t base = smem_addr(xs);
         for (int e = threadIdx.x; e < (t1 - t0) * (PT_ROWS / 4); e += PT_THREADS) {
@@ -456,31 +472,59 @@ template <int TOKENS> int launch_many_rows_of(int group, const CUtensorMap& map_
 
 using namespace chibi;
 
+// How many clusters of `splits` CTAs run at once (0: an error); CudaKernels.packed_cut asks.
+CHIBI_API int chibi_packed_many_rows_clusters(int splits)
+{
+    using T = PackedTile<192, 1>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)splits);
+    cfg.blockDim = dim3(PT_THREADS);
+    cfg.dynamicSmemBytes = T::SMEM;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (splits < 1 || splits > 8
+        || cudaFuncSetAttribute(packed_many_rows_kernel<192, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM) != cudaSuccess
+        || cudaOccupancyMaxActiveClusters(&clusters, packed_many_rows_kernel<192, 1>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return clusters;
+}
+
 // out[m, n] = x[m, k] times the matrix (+ residual); pair: act(x gate) * (x up), n features.  `tokens`: rows of x of a tile;
-// `splits`: CTAs that share a tile's columns.  CHIBI_ERR_UNSUPPORTED where x's rows do not start on 16 bytes.
+// every CTA takes `rounds` whole tiles, what is left is shared by clusters of `splits` CTAs, `clusters` of them (splits 1: CTAs).
+// CHIBI_ERR_UNSUPPORTED where x's rows do not start on 16 bytes.
 CHIBI_API int chibi_packed_many_rows(const void* data, int group, int n, int k, int pair, const void* x, long long x_stride, int m, void* out,
                                      int out_type, long long out_stride, const void* residual, long long residual_stride, int act,
-                                     int tokens, int splits, void* error, void* stream)
+                                     int tokens, int rounds, int splits, int clusters, void* error, void* stream)
 {
     if (!data || !x || !out || n < 1 || k < 1 || m < 1 || !packed_group_ok(group) || (out_type != CHIBI_F32 && out_type != CHIBI_BF16)
         || (pair && (residual || (act != 1 && act != 2))))
         return CHIBI_ERR_ARGUMENT;
     const int chunks = (k + PACKED_COLS - 1) / PACKED_COLS;
-    if ((tokens != 48 && tokens != 96 && tokens != 192) || splits < 1 || splits > 8 || splits > chunks)
+    if ((tokens != 48 && tokens != 96 && tokens != 192) || splits < 1 || splits > 8 || splits > chunks || rounds < 0
+        || clusters < 1)
         return CHIBI_ERR_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(x) & 15) || x_stride % 8)
         return CHIBI_ERR_UNSUPPORTED;
     const int each = pair ? PACKED_ROWS / 2 : PACKED_ROWS, tile_rows = pair ? PT_ROWS / 2 : PT_ROWS;
     const long long token_tiles = (m + (long long)tokens - 1) / tokens, tiles = (n + (long long)tile_rows - 1) / tile_rows * token_tiles;
-    if (tiles * splits > 0x7fffffff)
+    if (tiles > 0x3fffffff)
         return CHIBI_ERR_UNSUPPORTED;
+    const long long whole = (long long)rounds * clusters * splits;
+    if (splits > 1 ? tiles < whole || tiles - whole > clusters : tiles > whole)
+        return CHIBI_ERR_ARGUMENT;             // the pieces are not all tiles, each once
     CUtensorMap map_w, map;
     if (!packed_map(data, group, (n + each - 1) / each, chunks, 1, PT_ROWS / PACKED_ROWS, &map_w) || !tensor_map_2d(x, m, k, x_stride, tokens, &map))
         return CHIBI_ERR_UNSUPPORTED;
     const PackedProduct p { chunks, n, pair, m, out, out_type, out_stride, (const float*)residual,
-                            residual_stride, act, splits, (int)tiles, (int)token_tiles, (int*)error };
-    const int sms = device_sm_count();
-    const int ctas = splits > 1 ? (int)tiles * splits : (int)(tiles < sms ? tiles : sms);
+                            residual_stride, act, rounds, splits, (int)tiles, (int)token_tiles, (int*)error };
+    const int ctas = clusters * splits;
     return tokens == 48 ? launch_many_rows_of<48>(group, map_w, map, p, ctas, (cudaStream_t)stream)
                         : (tokens == 96 ? launch_many_rows_of<96>(group, map_w, map, p, ctas, (cudaStream_t)stream)
                                         : launch_many_rows_of<192>(group, map_w, map, p, ctas, (cudaStream_t)stream));

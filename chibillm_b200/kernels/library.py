@@ -106,7 +106,8 @@ _SIGNATURES = {
         "chibi_pack_weights": [P, P, I, I, I, L, L, I, P, P],
         "chibi_pack_codes": [P, P, P, P, I, I, L, L, L, L, I, P, P],
         "chibi_unpack_weights": [P, I, I, I, I, P, I, L, P],
-        "chibi_packed_many_rows": [P, I, I, I, I, P, L, I, P, I, L, P, L, I, I, I, P, P],
+        "chibi_packed_many_rows": [P, I, I, I, I, P, L, I, P, I, L, P, L, I, I, I, I, I, P, P],
+        "chibi_packed_many_rows_clusters": [I],
         "chibi_packed_few_rows_kb": [I, I, I, I, I, I, I, I, I],
         "chibi_packed_few_rows_clusters": [I, I, I, I, I, I],
         "chibi_packed_few_rows": [P, I, I, I, I, P, I, L, I, P, I, L, P, L, I, I, I, I, I, I, I, I, I, P, P],

@@ -14,7 +14,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import library
-from .packed import GROUPS, FewRowsPlan, PackedWeights, few_rows_plan, many_rows_cut
+from .packed import GROUPS, FewRowsPlan, ManyRowsCut, PackedWeights, few_rows_plan, many_rows_cut
 from ..csrc import build
 
 F32, BF16 = 0, 1
@@ -182,6 +182,8 @@ class CudaKernels:
         # matrices in 4 bits: up to so many bfloat16 rows of x stream the matrix once through mma.sync, more go to tcgen05
         self.packed_few_rows_max = 16
         self._packed_plans: Dict[tuple, FewRowsPlan] = {}
+        self._packed_cuts: Dict[tuple, ManyRowsCut] = {}
+        self._packed_clusters: Optional[list] = None
         self._partial_bufs = [None, None]
         self._partial_turn = 0
         self._partial_stamps = [0, 0]     # how often each of the two arrays has been handed out
@@ -884,6 +886,19 @@ class CudaKernels:
             self._packed_plans[key] = plan
         return plan
 
+    def packed_cut(self, w: PackedWeights, m: int) -> ManyRowsCut:
+        """The same for many rows of x."""
+        key = (w.rows, w.columns, w.paired, m)
+        cut = self._packed_cuts.get(key)
+        if cut is None:
+            if self._packed_clusters is None:
+                self._packed_clusters = [0] + [self.lib.chibi_packed_many_rows_clusters(s) for s in range(1, 9)]
+            cut = many_rows_cut(w.rows, w.columns, w.paired, m, lambda splits: self._packed_clusters[splits])
+            if len(self._packed_cuts) > 4096:
+                self._packed_cuts.clear()
+            self._packed_cuts[key] = cut
+        return cut
+
     def _packed_product(self, x, w: PackedWeights, out: torch.Tensor, residual: Optional[torch.Tensor], kind: Optional[str],
                         what: str) -> None:
         if isinstance(x, ScaledRows):
@@ -908,7 +923,7 @@ class CudaKernels:
                 status = self.lib.chibi_packed_many_rows(
                     _ptr(w.data), w.group, w.rows, w.columns, int(w.paired), _ptr(x), x.stride(0), M, _ptr(out), out_code, out.stride(0),
                     _ptr(residual), residual.stride(0) if residual is not None else 0, self.ACTIVATIONS[kind] if kind else 0,
-                    *many_rows_cut(w.rows, w.columns, w.paired, M, self.sm_count), _ptr(self.error), self._stream())
+                    *self.packed_cut(w, M), _ptr(self.error), self._stream())
                 if status != -2:
                     _check(status, what)
                     self.launches += 1

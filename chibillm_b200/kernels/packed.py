@@ -100,9 +100,37 @@ def few_rows_plan(rows: int, columns: int, paired: bool, m: int, smem_kb: Callab
     return None
 
 
-def many_rows_cut(rows: int, columns: int, paired: bool, m: int, sms: int) -> Tuple[int, int]:
-    """(rows of x of a tile, CTAs that share a tile's columns) of the product with many rows of x."""
+class ManyRowsCut(NamedTuple):
+    """See chibi_packed_many_rows in csrc/packed_tcgen05.cu."""
+    tokens: int
+    rounds: int
+    splits: int
+    clusters: int
+
+
+def many_rows_cut(rows: int, columns: int, paired: bool, m: int, most_clusters: Callable[[int], int]) -> ManyRowsCut:
+    """How tiles of the product with many rows of x are shared out: whole rounds of tiles on all SMs, what is left by clusters
+    whose CTAs share a tile's columns.  ``most_clusters(splits)``: how many clusters of so many CTAs run at once (the larger
+    they are, the fewer SMs they reach)."""
     tokens = 48 if m <= 48 else 96 if m <= 96 else 192
     tiles = -(-rows // (64 if paired else 128)) * -(-m // tokens)
     chunks = -(-columns // BLOCK_COLS)
-    return tokens, max(1, min(8, sms // tiles, chunks // 2))
+    best = None
+    for splits in range(1, min(8, chunks) + 1):
+        clusters = most_clusters(splits)
+        if clusters < 1:
+            continue
+        if splits == 1:
+            clusters = min(clusters, tiles)
+            cost, cut = -(-tiles // clusters) * chunks, ManyRowsCut(tokens, -(-tiles // clusters), 1, clusters)
+        else:
+            rounds, left = divmod(tiles, clusters * splits)
+            if left == 0 or left > clusters:
+                continue
+            if rounds == 0:
+                clusters = left
+            # (adding a shared tile's sums up costs about as much as three blocks of columns)
+            cost, cut = rounds * chunks + -(-chunks // splits) + 3, ManyRowsCut(tokens, rounds, splits, clusters)
+        if best is None or cost < best[0]:
+            best = (cost, cut)
+    return best[1]
