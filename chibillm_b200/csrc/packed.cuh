@@ -19,6 +19,20 @@
 #include "common.cuh"
 #include "tensor_map.cuh"
 
+#include <atomic>
+
+// What stays the same from call to call of a product with such a matrix: made once for a number of rows and the types
+// (library.py has the same fields).
+struct ChibiPackedCall {
+    const void* data;
+    void* error;
+    int group, n, k, pair;           // n: rows of the matrix, of a pair its features
+    int m, x_type, out_type, act;    // act (pairs): 1 gelu with tanh, 2 silu
+    int splits, clusters, tokens;    // both kernels
+    int warps, along_k, batch, depth, run;         // few rows
+    int rounds;                      // many rows
+};
+
 namespace chibi {
 
 constexpr int PACKED_ROWS = 32, PACKED_COLS = 128, PACKED_CODE_BYTES = PACKED_ROWS * PACKED_COLS / 2;
@@ -39,6 +53,24 @@ __host__ __device__ constexpr int packed_side(int pair, int r) { return pair ? (
 __host__ __device__ constexpr int packed_source_row(int pair, int rb, int r)
 {
     return pair ? rb * (PACKED_ROWS / 2) + (r >> 4) * 8 + (r & 7) : rb * PACKED_ROWS + r;
+}
+
+// Lets `kernel` have so much shared memory; asked of each device once.
+template <typename K> inline cudaError_t packed_allow_shared(K kernel, std::atomic<unsigned long long>& allowed, size_t bytes)
+{
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess)
+        return e;
+    const unsigned long long bit = 1ull << (device & 63);
+    if (device < 64 && (allowed.load(std::memory_order_relaxed) & bit))
+        return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess)
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    else
+        cudaGetLastError();
+    return e;
 }
 
 // A tensor map over the records: a box is `box_cols` neighbouring records of each of `box_rows` blocks of rows, and lands record

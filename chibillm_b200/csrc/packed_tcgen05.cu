@@ -450,13 +450,15 @@ template <int TOKENS, int GROUP_BLOCKS>
 int launch_many_rows(const CUtensorMap& map_w, const CUtensorMap& map, const PackedProduct& p, int ctas, cudaStream_t stream)
 {
     constexpr size_t SMEM = PackedTile<TOKENS, GROUP_BLOCKS>::SMEM;
-    const cudaError_t e = cudaFuncSetAttribute(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)SMEM);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
+    static std::atomic<unsigned long long> allowed;
+    const cudaError_t e = packed_allow_shared(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, allowed, SMEM);
+    if (e != cudaSuccess)
         return (int)e;
-    }
-    launch_cluster_x(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, dim3((unsigned)ctas), dim3(PT_THREADS), SMEM, stream, p.splits, map_w, map, p);
+    const dim3 grid((unsigned)ctas), block(PT_THREADS);
+    if (p.splits > 1)
+        launch_cluster_x(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, grid, block, SMEM, stream, p.splits, map_w, map, p);
+    else
+        launch(packed_many_rows_kernel<TOKENS, GROUP_BLOCKS>, grid, block, SMEM, stream, map_w, map, p);
     return launch_status();
 }
 
@@ -499,33 +501,33 @@ CHIBI_API int chibi_packed_many_rows_clusters(int splits)
 // out[m, n] = x[m, k] times the matrix (+ residual); pair: act(x gate) * (x up), n features.  `tokens`: rows of x of a tile;
 // every CTA takes `rounds` whole tiles, what is left is shared by clusters of `splits` CTAs, `clusters` of them (splits 1: CTAs).
 // CHIBI_ERR_UNSUPPORTED where x's rows do not start on 16 bytes.
-CHIBI_API int chibi_packed_many_rows(const void* data, int group, int n, int k, int pair, const void* x, long long x_stride, int m, void* out,
-                                     int out_type, long long out_stride, const void* residual, long long residual_stride, int act,
-                                     int tokens, int rounds, int splits, int clusters, void* error, void* stream)
+CHIBI_API int chibi_packed_many_rows(const ChibiPackedCall* c, const void* x, long long x_stride, void* out, long long out_stride,
+                                     const void* residual, long long residual_stride, void* stream)
 {
-    if (!data || !x || !out || n < 1 || k < 1 || m < 1 || !packed_group_ok(group) || (out_type != CHIBI_F32 && out_type != CHIBI_BF16)
-        || (pair && (residual || (act != 1 && act != 2))))
+    if (!c || !c->data || !x || !out || c->n < 1 || c->k < 1 || c->m < 1 || !packed_group_ok(c->group) || c->x_type != CHIBI_BF16
+        || (c->out_type != CHIBI_F32 && c->out_type != CHIBI_BF16) || (c->pair && (residual || (c->act != 1 && c->act != 2))))
         return CHIBI_ERR_ARGUMENT;
-    const int chunks = (k + PACKED_COLS - 1) / PACKED_COLS;
-    if ((tokens != 48 && tokens != 96 && tokens != 192) || splits < 1 || splits > 8 || splits > chunks || rounds < 0
-        || clusters < 1)
+    const int chunks = (c->k + PACKED_COLS - 1) / PACKED_COLS, tokens = c->tokens, splits = c->splits;
+    if ((tokens != 48 && tokens != 96 && tokens != 192) || splits < 1 || splits > 8 || splits > chunks || c->rounds < 0 || c->clusters < 1)
         return CHIBI_ERR_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(x) & 15) || x_stride % 8)
         return CHIBI_ERR_UNSUPPORTED;
-    const int each = pair ? PACKED_ROWS / 2 : PACKED_ROWS, tile_rows = pair ? PT_ROWS / 2 : PT_ROWS;
-    const long long token_tiles = (m + (long long)tokens - 1) / tokens, tiles = (n + (long long)tile_rows - 1) / tile_rows * token_tiles;
+    const int each = c->pair ? PACKED_ROWS / 2 : PACKED_ROWS, tile_rows = c->pair ? PT_ROWS / 2 : PT_ROWS;
+    const long long token_tiles = (c->m + (long long)tokens - 1) / tokens, tiles = (c->n + (long long)tile_rows - 1) / tile_rows * token_tiles;
     if (tiles > 0x3fffffff)
         return CHIBI_ERR_UNSUPPORTED;
-    const long long whole = (long long)rounds * clusters * splits;
-    if (splits > 1 ? tiles < whole || tiles - whole > clusters : tiles > whole)
+    const long long whole = (long long)c->rounds * c->clusters * splits;
+    if (splits > 1 ? tiles < whole || tiles - whole > c->clusters : tiles > whole)
         return CHIBI_ERR_ARGUMENT;             // the pieces are not all tiles, each once
     CUtensorMap map_w, map;
-    if (!packed_map(data, group, (n + each - 1) / each, chunks, 1, PT_ROWS / PACKED_ROWS, &map_w) || !tensor_map_2d(x, m, k, x_stride, tokens, &map))
+    if (!packed_map(c->data, c->group, (c->n + each - 1) / each, chunks, 1, PT_ROWS / PACKED_ROWS, &map_w)
+        || !tensor_map_2d(x, c->m, c->k, x_stride, tokens, &map))
         return CHIBI_ERR_UNSUPPORTED;
-    const PackedProduct p { chunks, n, pair, m, out, out_type, out_stride, (const float*)residual,
-                            residual_stride, act, rounds, splits, (int)tiles, (int)token_tiles, (int*)error };
-    const int ctas = clusters * splits;
-    return tokens == 48 ? launch_many_rows_of<48>(group, map_w, map, p, ctas, (cudaStream_t)stream)
-                        : (tokens == 96 ? launch_many_rows_of<96>(group, map_w, map, p, ctas, (cudaStream_t)stream)
-                                        : launch_many_rows_of<192>(group, map_w, map, p, ctas, (cudaStream_t)stream));
+    const PackedProduct p { chunks, c->n, c->pair, c->m, out, c->out_type, out_stride, (const float*)residual, residual_stride, c->act,
+                            c->rounds, splits, (int)tiles, (int)token_tiles, (int*)c->error };
+    const int ctas = c->clusters * splits;
+    const cudaStream_t s = (cudaStream_t)stream;
+    return tokens == 48 ? launch_many_rows_of<48>(c->group, map_w, map, p, ctas, s)
+                        : (tokens == 96 ? launch_many_rows_of<96>(c->group, map_w, map, p, ctas, s)
+                                        : launch_many_rows_of<192>(c->group, map_w, map, p, ctas, s));
 }

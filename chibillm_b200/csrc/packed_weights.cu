@@ -635,36 +635,37 @@ CHIBI_API int chibi_packed_few_rows_clusters(int x32, int group, int tokens, int
 }
 
 // out[m, n] = x[m, k] times the matrix (+ residual); pair: act(x gate) * (x up), n features.  The plan: see FewRows.
-CHIBI_API int chibi_packed_few_rows(const void* data, int group, int n, int k, int pair, const void* x, int x_type, long long x_stride,
-                                    int m, void* out, int out_type, long long out_stride, const void* residual,
-                                    long long residual_stride, int act, int warps, int splits, int along_k, int batch, int depth, int run,
-                                    int tokens, int clusters, void* error, void* stream)
+CHIBI_API int chibi_packed_few_rows(const ChibiPackedCall* c, const void* x, long long x_stride, void* out, long long out_stride,
+                                    const void* residual, long long residual_stride, void* stream)
 {
-    if (!data || !x || !out || n < 1 || k < 1 || m < 1 || !packed_group_ok(group) || (x_type != CHIBI_F32 && x_type != CHIBI_BF16)
-        || (out_type != CHIBI_F32 && out_type != CHIBI_BF16) || (pair && (residual || (act != 1 && act != 2))))
+    if (!c || !c->data || !x || !out || c->n < 1 || c->k < 1 || c->m < 1 || !packed_group_ok(c->group)
+        || (c->x_type != CHIBI_F32 && c->x_type != CHIBI_BF16) || (c->out_type != CHIBI_F32 && c->out_type != CHIBI_BF16)
+        || (c->pair && (residual || (c->act != 1 && c->act != 2))))
         return CHIBI_ERR_ARGUMENT;
-    const int chunks = (k + PACKED_COLS - 1) / PACKED_COLS;
-    if ((warps != 8 && warps != 16) || splits < 1 || splits > 8 || (splits & (splits - 1)) || splits > chunks || along_k < 1
-        || along_k > warps || (along_k & (along_k - 1)) || batch < 1 || depth < 1 || run < 1 || tokens < 1 || tokens > warps || clusters < 1)
+    const int chunks = (c->k + PACKED_COLS - 1) / PACKED_COLS;
+    if ((c->warps != 8 && c->warps != 16) || c->splits < 1 || c->splits > 8 || (c->splits & (c->splits - 1)) || c->splits > chunks
+        || c->along_k < 1 || c->along_k > c->warps || (c->along_k & (c->along_k - 1)) || c->batch < 1 || c->depth < 1 || c->run < 1
+        || c->run > 256 || c->tokens < 1 || c->tokens > c->warps || c->clusters < 1)
         return CHIBI_ERR_ARGUMENT;
-    const bool x32 = x_type == CHIBI_F32;
-    const size_t smem = few_rows_smem(x32, group, chunks, warps, splits, batch, depth, run, tokens);
-    const long long token_blocks = ((long long)m + tokens - 1) / tokens;
-    const int each = pair ? PACKED_ROWS / 2 : PACKED_ROWS;
-    if (smem > FEW_SMEM_LIMIT || token_blocks > 65535)
-        return CHIBI_ERR_UNSUPPORTED;
+    const bool x32 = c->x_type == CHIBI_F32;
+    const size_t smem = few_rows_smem(x32, c->group, chunks, c->warps, c->splits, c->batch, c->depth, c->run, c->tokens);
+    const long long token_blocks = ((long long)c->m + c->tokens - 1) / c->tokens;
+    const int each = c->pair ? PACKED_ROWS / 2 : PACKED_ROWS, row_blocks = (c->n + each - 1) / each;
     CUtensorMap map;
-    if (run > 256 || !packed_map(data, group, (n + each - 1) / each, chunks, run, 1, &map))
+    if (smem > FEW_SMEM_LIMIT || token_blocks > 65535 || !packed_map(c->data, c->group, row_blocks, chunks, c->run, 1, &map))
         return CHIBI_ERR_UNSUPPORTED;
-    const FewRows p { (n + each - 1) / each, chunks, n, k, pair, x, x_stride, m, out, out_type, out_stride,
-                      (const float*)residual, residual_stride, act, warps, splits, along_k, batch, depth, run, tokens, clusters, (int*)error };
-    void (*kernel)(const CUtensorMap, const FewRows) = few_rows_kernel(x32, tokens, group);
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SMEM_LIMIT);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
+    const FewRows p { row_blocks, chunks, c->n, c->k, c->pair, x, x_stride, c->m, out, c->out_type, out_stride, (const float*)residual,
+                      residual_stride, c->act, c->warps, c->splits, c->along_k, c->batch, c->depth, c->run, c->tokens, c->clusters,
+                      (int*)c->error };
+    void (*kernel)(const CUtensorMap, const FewRows) = few_rows_kernel(x32, c->tokens, c->group);
+    static std::atomic<unsigned long long> allowed[2][2][3];
+    const cudaError_t e = packed_allow_shared(kernel, allowed[x32][c->tokens <= 8][c->group / 64], FEW_SMEM_LIMIT);
+    if (e != cudaSuccess)
         return (int)e;
-    }
-    launch_cluster_x(kernel, dim3((unsigned)(clusters * splits), (unsigned)token_blocks), dim3((unsigned)warps * 32), smem,
-                     (cudaStream_t)stream, splits, map, p);
+    const dim3 grid((unsigned)(c->clusters * c->splits), (unsigned)token_blocks), block((unsigned)c->warps * 32);
+    if (c->splits > 1)
+        launch_cluster_x(kernel, grid, block, smem, (cudaStream_t)stream, c->splits, map, p);
+    else
+        launch(kernel, grid, block, smem, (cudaStream_t)stream, map, p);
     return launch_status();
 }

@@ -106,11 +106,11 @@ _SIGNATURES = {
         "chibi_pack_weights": [P, P, I, I, I, L, L, I, P, P],
         "chibi_pack_codes": [P, P, P, P, I, I, L, L, L, L, I, P, P],
         "chibi_unpack_weights": [P, I, I, I, I, P, I, L, P],
-        "chibi_packed_many_rows": [P, I, I, I, I, P, L, I, P, I, L, P, L, I, I, I, I, I, P, P],
+        "chibi_packed_many_rows": [P, P, L, P, L, P, L, P],
         "chibi_packed_many_rows_clusters": [I],
         "chibi_packed_few_rows_kb": [I, I, I, I, I, I, I, I, I],
         "chibi_packed_few_rows_clusters": [I, I, I, I, I, I],
-        "chibi_packed_few_rows": [P, I, I, I, I, P, I, L, I, P, I, L, P, L, I, I, I, I, I, I, I, I, I, P, P],
+        "chibi_packed_few_rows": [P, P, L, P, L, P, L, P],
         "chibi_decayed_attention": [P, I, L, I, P, P, P, P, L, P, P, L, I, I, I, I, I, I, P],
     },
     "chibi_attention_tc": {
@@ -141,6 +141,13 @@ class NormOut(ctypes.Structure):
     """ChibiNormOut of gemm_tcgen05.cu: the norm output that a product writes beside the residual."""
     _fields_ = [("w", c_void_p), ("w_type", c_int), ("offset", c_float), ("out", c_void_p),
                 ("out_stride", c_longlong), ("ssq", c_void_p), ("ssq_floats", c_longlong)]
+
+
+class PackedCall(ctypes.Structure):
+    """ChibiPackedCall of packed.cuh: what stays the same from call to call of a product with a matrix in 4 bits."""
+    _fields_ = [("data", c_void_p), ("error", c_void_p)] + [(name, c_int) for name in (
+        "group", "n", "k", "pair", "m", "x_type", "out_type", "act", "splits", "clusters", "tokens", "warps", "along_k", "batch", "depth",
+        "run", "rounds")]
 
 
 class HeadsOut(ctypes.Structure):

@@ -180,7 +180,7 @@ class CudaKernels:
         self._attention_tied_libs = {}
         self.use_tcgen05_attention = True
         # matrices in 4 bits: up to so many bfloat16 rows of x stream the matrix once through mma.sync, more go to tcgen05
-        self.packed_few_rows_max = 16
+        self.packed_few_rows_max = 12
         self._packed_plans: Dict[tuple, FewRowsPlan] = {}
         self._packed_cuts: Dict[tuple, ManyRowsCut] = {}
         self._packed_clusters: Optional[list] = None
@@ -854,9 +854,10 @@ class CudaKernels:
         return torch.cuda.device(self._device_index)
 
     def _on_this_device(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
-        _need_cuda(*tensors)
         for t in tensors:
-            if t is not None and t.device.index != self._device_index:
+            if t is not None and not t.is_cuda:
+                _need_cuda(t)
+            if t is not None and t.get_device() != self._device_index:
                 raise KernelError(f"{what}: a tensor on {t.device}, these kernels run on cuda:{self._device_index}")
 
     def _packed_sizes(self, w: torch.Tensor, group: int, what: str) -> None:
@@ -876,9 +877,9 @@ class CudaKernels:
         plan = self._packed_plans.get(key)
         if plan is None:
             lib, x = self.lib, int(x32)
-            plan = few_rows_plan(w.rows, w.columns, w.paired, m,
+            plan = few_rows_plan(w.rows, w.columns, w.paired, m, x32,
                                  lambda *cut: lib.chibi_packed_few_rows_kb(x, w.group, w.columns, *cut),
-                                 lambda *cut: lib.chibi_packed_few_rows_clusters(x, w.group, *cut))
+                                 lambda *cut: lib.chibi_packed_few_rows_clusters(x, w.group, *cut), self.sm_count)
             if plan is None:
                 raise KernelError(f"a product over {w.columns} columns in 4 bits: more than the kernel holds")
             if len(self._packed_plans) > 4096:
@@ -899,6 +900,14 @@ class CudaKernels:
             self._packed_cuts[key] = cut
         return cut
 
+    def _packed_call(self, w: PackedWeights, m: int, x_code: int, out_code: int, kind: Optional[str], many: bool):
+        """The arguments of a product that stay the same from call to call."""
+        call = library.PackedCall(_ptr(w.data), _ptr(self.error), w.group, w.rows, w.columns, int(w.paired), m, x_code, out_code,
+                                  self.ACTIVATIONS[kind] if kind else 0)
+        for name, value in (self.packed_cut(w, m) if many else self.packed_plan(w, m, x_code == F32))._asdict().items():
+            setattr(call, name, value)
+        return ctypes.pointer(call)
+
     def _packed_product(self, x, w: PackedWeights, out: torch.Tensor, residual: Optional[torch.Tensor], kind: Optional[str],
                         what: str) -> None:
         if isinstance(x, ScaledRows):
@@ -906,36 +915,37 @@ class CudaKernels:
         if w.paired != (kind is not None):
             raise KernelError(f"{what}: a pair of matrices (pack_gate_up) belongs to linear_swiglu, any other to linear")
         self._on_this_device(what, x, w.data, out, residual)
-        _rows_contiguous(x, f"{what}: x")
-        _rows_contiguous(out, f"{what}: out")
+        _rows_contiguous(x, what)
+        _rows_contiguous(out, what)
         M, K = x.shape
         if K != w.columns or out.shape != (M, w.rows):
             raise KernelError(f"{what}: shapes x {tuple(x.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
         if residual is not None:
-            _rows_contiguous(residual, f"{what}: residual")
+            _rows_contiguous(residual, what)
             if residual.dtype != torch.float32 or residual.shape != out.shape:
                 raise KernelError(f"{what}: residual must be float32 [M, N]")
         x_code, out_code = _code(x), _code(out)
         if M == 0:
             return
-        with self._current_device():
-            if x_code == BF16 and M > self.packed_few_rows_max:
-                status = self.lib.chibi_packed_many_rows(
-                    _ptr(w.data), w.group, w.rows, w.columns, int(w.paired), _ptr(x), x.stride(0), M, _ptr(out), out_code, out.stride(0),
-                    _ptr(residual), residual.stride(0) if residual is not None else 0, self.ACTIVATIONS[kind] if kind else 0,
-                    *self.packed_cut(w, M), _ptr(self.error), self._stream())
-                if status != -2:
-                    _check(status, what)
-                    self.launches += 1
-                    self.tensor_core_calls += 1
-                    return
-            plan = self.packed_plan(w, M, x_code == F32)
+        if torch.cuda.current_device() != self._device_index:
+            with torch.cuda.device(self._device_index):
+                return self._packed_product(x, w, out, residual, kind, what)
+        rest = (_ptr(x), x.stride(0), _ptr(out), out.stride(0), _ptr(residual), residual.stride(0) if residual is not None else 0,
+                self._stream())
+        for many in ((True, False) if x_code == BF16 and M > self.packed_few_rows_max else (False,)):
+            key = (self, w.data.data_ptr(), M, x_code, out_code, kind, many)
+            call = w.calls.get(key)
+            if call is None:
+                if len(w.calls) > 256:
+                    w.calls.clear()
+                call = w.calls[key] = self._packed_call(w, M, x_code, out_code, kind, many)
+            status = (self.lib.chibi_packed_many_rows if many else self.lib.chibi_packed_few_rows)(call, *rest)
+            if many and status == -2:
+                continue                 # rows of x that a tile copy cannot fetch
+            _check(status, what)
             self.launches += 1
             self.tensor_core_calls += 1
-            _check(self.lib.chibi_packed_few_rows(
-                _ptr(w.data), w.group, w.rows, w.columns, int(w.paired), _ptr(x), x_code, x.stride(0), M, _ptr(out), out_code, out.stride(0),
-                _ptr(residual), residual.stride(0) if residual is not None else 0, self.ACTIVATIONS[kind] if kind else 0,
-                *plan, _ptr(self.error), self._stream()), what)
+            return
 
     def qk_norm_rope_append(self, qkv: torch.Tensor, q_out: torch.Tensor,
                             k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],

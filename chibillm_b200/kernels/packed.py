@@ -26,6 +26,7 @@ class PackedWeights:
 
     def __init__(self, data: torch.Tensor, rows: int, columns: int, group: int, paired: bool):
         self.data, self.rows, self.columns, self.group, self.paired = data, rows, columns, group, paired
+        self.calls = {}              # (kernels, rows of x, types, activation) -> the arguments that stay the same
 
     @property
     def shape(self) -> torch.Size:
@@ -53,19 +54,27 @@ class FewRowsPlan(NamedTuple):
     clusters: int
 
 
-def few_rows_plan(rows: int, columns: int, paired: bool, m: int, smem_kb: Callable[..., int],
-                  most_clusters: Callable[[int, int, int, int], int]) -> Optional[FewRowsPlan]:
-    """How CTAs and warps share a product of m rows of x.  ``smem_kb(tokens, warps, splits, batch, depth, run)`` is a CTA's
-    shared memory, ``most_clusters(tokens, warps, splits, kb)`` how many clusters run at once.  None if nothing fits."""
+def few_rows_plan(rows: int, columns: int, paired: bool, m: int, wide: bool, smem_kb: Callable[..., int],
+                  most_clusters: Callable[[int, int, int, int], int], sms: int) -> Optional[FewRowsPlan]:
+    """How CTAs and warps share a product of m rows of x (``wide``: 32-bit ones).  ``smem_kb(tokens, warps, splits, batch, depth,
+    run)`` is a CTA's shared memory, ``most_clusters(tokens, warps, splits, kb)`` how many clusters run at once.  None if nothing fits.
+
+    The cut with the least time by a rough model, in ns, fitted to sweeps of all cuts (1 to 16 rows of x, matrices of 2,048 x 1,024
+    to 151,936 x 4,096): a record takes an SM 60 and a warp 530 (what instructions it issues, and their latency), two instructions
+    for every 8 rows of x more of it; adding up the sums of a round 400; a cluster that adds up across CTAs 1,200.  About 64
+    records are to be on their way to an SM (at 32, 4,096 x 12,288 took 13.3 us instead of 10.2), and no more room is taken than
+    a warp's records need, so that the next kernel's CTAs fit beside (2,051 x 1,021: 6.2 us with four places a warp, 4.4 with one)."""
     blocks = -(-rows // (BLOCK_ROWS // 2 if paired else BLOCK_ROWS))
     chunks = -(-columns // BLOCK_COLS)
     tokens = -(-m // -(-m // FEW_TOKENS))
     while tokens >= 1:
         best = None
         token_blocks = -(-m // tokens)
-        for warps, room in ((8, FEW_SMEM_KB // 2), (16, FEW_SMEM_KB)):
+        issue = 60 * (1.4 if tokens > 8 else 1.0) * (1.5 if wide else 1.0)
+        for warps, resident in ((8, 2), (8, 1), (16, 1)):
             if tokens > warps:
                 continue
+            room = FEW_SMEM_KB // resident
             for splits in (1, 2, 4, 8):
                 if splits > chunks:
                     break
@@ -75,21 +84,23 @@ def few_rows_plan(rows: int, columns: int, paired: bool, m: int, smem_kb: Callab
                         continue
                     per_unit = warps // along_k
                     each = -(-mine // along_k)
-                    run = min(2, each)
-                    for depth in (4, 3, 2):
-                        if smem_kb(tokens, warps, splits, 1, depth, run) <= room:
-                            break
-                    else:
-                        continue
-                    at_once = most_clusters(tokens, warps, splits, smem_kb(tokens, warps, splits, 1, depth, run))
-                    if at_once < 1:
-                        continue
                     units = -(-blocks // per_unit)
-                    clusters = min(units, max(1, at_once // token_blocks))
+                    run = max(r for r in ((1, 2, 3, 4) if warps * resident == 8 else (1, 2)) if each % r == 0)
+                    rounds = -(-units // max(1, min(units, resident * sms // splits // token_blocks)))
+                    depth = min(-(-64 // (warps * resident * run)), rounds * (each // run))
+                    while depth > 1 and smem_kb(tokens, warps, splits, 1, depth, run) > room:
+                        depth -= 1
+                    kb = smem_kb(tokens, warps, splits, 1, depth, run)
+                    if kb > room:
+                        continue
+                    clusters = min(units, max(1, most_clusters(tokens, warps, splits, kb) // token_blocks))
                     rounds = -(-units // clusters)
-                    cost = rounds * (per_unit * mine + 2) * (2 if warps == 8 and clusters * splits > 148 else 1) + (20 if splits > 1 else 0)
-                    if best is None or cost < best[0]:
-                        best = (cost, FewRowsPlan(warps, splits, along_k, 1, depth, run, tokens, clusters), rounds, room)
+                    on_sm = -(-clusters * splits // sms)
+                    busy = on_sm * per_unit * min(along_k, mine)
+                    time = on_sm * rounds * per_unit * mine * max(issue, 530 / busy) + rounds * 400 + (1200 if splits > 1 else 0) \
+                        + mine * 16 * tokens / (warps * 32) * 30
+                    if best is None or time < best[0]:
+                        best = (time, FewRowsPlan(warps, splits, along_k, 1, depth, run, tokens, clusters), rounds, room)
         if best is not None:
             _, plan, rounds, room = best
             batch = 1

@@ -33,7 +33,7 @@ _NOT_LAUNCHES = ("chibi_gemm_bf16_splits", "chibi_gemm_bf16_splits_capped", "chi
 # where M, N, K stand among the arguments of the matrix products
 _PRODUCT_SIZES = {"chibi_gemm_bf16": (5, 6, 7), "chibi_gemm_bf16_rows": (5, 6, 7), "chibi_gemm_bf16_fused": (5, 6, 7),
                   "chibi_gemm_bf16_partial": (2, 3, 4), "chibi_gemm_simt": (7, 8, 9),
-                  "chibi_gemm_f32": (4, 5, 6), "chibi_packed_few_rows": (8, 2, 3), "chibi_packed_many_rows": (7, 2, 3)}
+                  "chibi_gemm_f32": (4, 5, 6)}
 
 
 def launch_name(function: str, args: tuple) -> str:
@@ -41,6 +41,9 @@ def launch_name(function: str, args: tuple) -> str:
     products, the weight's shape and whether few (<= 64), up to 128 (where the narrow
     products still run the few-row kernel) or many rows ran."""
     name = function[6:] if function.startswith("chibi_") else function
+    if function in ("chibi_packed_few_rows", "chibi_packed_many_rows"):
+        call = args[0].contents
+        return f"{name}{' (gated)' if call.pair else ''} {call.n}x{call.k}"
     where = _PRODUCT_SIZES.get(function)
     if where is not None:
         m, n, k = (int(args[i]) for i in where)
