@@ -20,13 +20,17 @@ class LLM:
     reference's command-line flags (src/cli_options.cc:13-25).  The defaults of
     the scheduler are sized for a B200 (64 requests, steps of 4,096 tokens, prompt
     portions of 1,024 while others wait or decode); the reference's own, sized for
-    a laptop GPU, are 4 requests, 128 tokens and 64 (src/scheduler.h:30-39)."""
+    a laptop GPU, are 4 requests, 128 tokens and 64 (src/scheduler.h:30-39).
+
+    ``weight_group`` (32, 64 or 128) puts the matrices of attention, of dense feed-forwards and of the output into 4 bits
+    while the model is loaded, with a bfloat16 scale for so many neighbouring columns of a row
+    (the reference's load-time ``--quantize q4``; here symmetric, without offsets)."""
 
     def __init__(self, model_dir: Optional[str], dtype: str = "bfloat16", device: str = "cuda:0",
                  context_length: int = 4096, kv_cache_tokens: Optional[int] = None,
                  max_sequences: int = 64, max_batch_tokens: int = 4096, prefill_chunk_tokens: int = 1024,
                  page_size: int = KV_PAGE_SIZE, kernels=None, random_config: Optional[dict] = None,
-                 random_seed: int = 0):
+                 random_seed: int = 0, weight_group: Optional[int] = None):
         if context_length <= 0 or context_length % page_size != 0:
             raise ValueError(f"context_length must be a positive multiple of {page_size}")
         pool = kv_cache_tokens if kv_cache_tokens is not None else context_length * max_sequences
@@ -37,11 +41,11 @@ class LLM:
         if model_dir is not None:
             self.runner = ModelRunner.from_folder(model_dir, dtype=dtype, device=device,
                                                   page_size=page_size, pool_tokens=pool,
-                                                  max_requests=max_sequences, kernels=kernels)
+                                                  max_requests=max_sequences, kernels=kernels, weight_group=weight_group)
         else:
             self.runner = ModelRunner.from_random(random_config, seed=random_seed, dtype=dtype,
                                                   device=device, page_size=page_size, pool_tokens=pool,
-                                                  max_requests=max_sequences, kernels=kernels)
+                                                  max_requests=max_sequences, kernels=kernels, weight_group=weight_group)
         self.context_length = min(context_length, self.runner.max_context_tokens)
         self.engine = InferenceEngine(self.runner, SchedulerConfig(
             max_sequences=max_sequences, max_batch_tokens=max_batch_tokens,

@@ -20,7 +20,8 @@ sequences, unless ``--kv-blocks`` says otherwise), one sequence and batches of
 
 Options the reference has and this engine does not build are refused by name:
 ``--serve`` and ``--kv-cache-tokens`` (HTTP server), ``--prompt-cache-mib``
-other than 0 (prefix cache), ``--quantize q4`` (quantized weights).
+other than 0 (prefix cache), ``--quantize q4`` (affine 4-bit weights; ``--weight-group`` is
+this engine's own form).
 """
 from __future__ import annotations
 
@@ -36,7 +37,8 @@ KV_BLOCK_SIZE = 16          # src/cli_options.h:15
 USAGE = """Usage: python -m chibillm_b200 [--context-length N] [--max-tokens N] [model-directory]
   --context-length N  Prompt + output capacity (default: 32768; multiple of the page size)
   --max-tokens N      Reply limit (default: 8192)
-  --quantize none     Only 'none': quantized weights are not built in this engine
+  --quantize none     Only 'none': the reference's affine 4-bit weights are not built in this engine
+  --weight-group G    Matrices in 4 bits with a scale for every G columns of a row (32, 64 or 128)
   --prompt-cache-mib 0  Only 0: the prefix cache is not built in this engine
   --no-stream         Print replies only when complete
   --progress=auto|off  Prefill progress on terminals (default: auto)
@@ -83,6 +85,7 @@ class CliOptions:
     prefill_chunk: int = 0           # 0: derived from max_seqs
     kv_block_size: int = KV_BLOCK_SIZE
     kv_blocks: int = 0               # 0: derived from the context length
+    weight_group: Optional[int] = None
     profile: bool = False
     profile_passes: bool = False
     help: bool = False
@@ -145,7 +148,12 @@ def parse_cli_options(argv: List[str]) -> CliOptions:
             if v not in ("none", "q4"):
                 raise CliError(f"invalid quantization: {v}")
             if v != "none":
-                raise CliError("--quantize q4: quantized weights are not built in this engine")
+                raise CliError("--quantize q4: affine 4-bit weights are not built in this engine (see --weight-group)")
+        elif arg == "--weight-group":
+            v = value(arg)
+            if v not in ("32", "64", "128"):
+                raise CliError(f"invalid weight group: {v} (32, 64 or 128)")
+            o.weight_group = int(v)
         elif arg == "--serve":
             raise CliError("--serve: the HTTP server is not built in this engine")
         elif arg == "--kv-cache-tokens":
@@ -280,7 +288,7 @@ def run(options: CliOptions, stdin=None, stdout=None, stderr=None, kernels=None,
                   kv_cache_tokens=pages * options.kv_block_size, max_sequences=options.max_seqs,
                   max_batch_tokens=options.max_batch_tokens, prefill_chunk_tokens=options.prefill_chunk,
                   page_size=options.kv_block_size, kernels=kernels, random_config=random_config,
-                  random_seed=options.weights_seed)
+                  random_seed=options.weights_seed, weight_group=options.weight_group)
     except ConfigError as e:
         what = ("unsupported model architecture in " if e.code == "unsupported_architecture"
                 else "failed to load model from ")

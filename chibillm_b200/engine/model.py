@@ -68,7 +68,8 @@ class DecoderModel:
     def bind(self, tensors: Dict[str, torch.Tensor]) -> None:
         s = self.spec
         self.embedding = tensors[s.embedding_name].contiguous()
-        self.output = tensors[s.output_name].contiguous() if s.output_name in tensors else self.embedding
+        # (a tied embedding stays as it is for its own rows and is kept a second time, in 4 bits, as the output matrix)
+        self.output = self.runtime.pack(tensors[s.output_name].contiguous() if s.output_name in tensors else self.embedding)
         self.final_norm.bind(tensors)
         for b in self.blocks:
             b.bind(tensors)

@@ -67,12 +67,14 @@ def main(argv=None) -> int:
                         help="most tokens that live requests hold at any time (the cache pool's size)")
     parser.add_argument("--page-size", type=int, default=16, help="tokens per cache page (default 16)")
     parser.add_argument("--max-requests", type=int, default=8, help="most live requests (default 8)")
+    parser.add_argument("--weight-group", type=int, default=None, choices=[32, 64, 128],
+                        help="matrices in 4 bits with a scale for so many columns of a row")
     parser.add_argument("--device", default="cuda:0")
     args = parser.parse_args(argv)
     if args.max_tokens <= 0 or args.page_size <= 0 or 64 % args.page_size != 0:
         parser.error("--max-tokens must be positive and --page-size must divide 64")
     runner = ModelRunner.from_folder(args.model, dtype=args.dtype, device=args.device,
                                      page_size=args.page_size, pool_tokens=args.max_tokens,
-                                     max_requests=args.max_requests)
+                                     max_requests=args.max_requests, weight_group=args.weight_group)
     replay(runner, iter(sys.stdin.readline, ""), args.out)
     return 0

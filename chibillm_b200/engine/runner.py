@@ -21,6 +21,7 @@ from ..cache import native
 from ..cache.manager import CacheError, CacheManager
 from ..cache.storage import CacheStorage, FixedStateView, plan_cache
 from ..config.registry import load_config
+from ..kernels.packed import GROUPS as WEIGHT_GROUPS
 from ..parts.base import Runtime
 from ..weights.loader import load_weights
 from .batch import BatchError, StepContext, StepEntry, Workspace
@@ -41,11 +42,13 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"dtype '{name}' is not supported (bfloat16 or float32)") from None
 
 
-def make_runtime(dtype, device="cuda:0", kernels=None, spec=None) -> Runtime:
+def make_runtime(dtype, device="cuda:0", kernels=None, spec=None, weight_group: Optional[int] = None) -> Runtime:
     """The product's runtime: a CUDA device and this package's kernels.  A test
     may pass a stand-in for the kernels (then any device is allowed).  With the
     model's ``spec`` the libraries it will load are built together first."""
     device = torch.device(device)
+    if weight_group is not None and weight_group not in WEIGHT_GROUPS:
+        raise ValueError(f"weight_group {weight_group}: matrices in 4 bits have groups of one of {WEIGHT_GROUPS} columns")
     if kernels is None:
         from ..kernels.ops import CudaKernels
         if spec is not None:
@@ -71,7 +74,9 @@ def make_runtime(dtype, device="cuda:0", kernels=None, spec=None) -> Runtime:
                         head_dims.add(m.head_dim)
             build.prepare(head_dims, bfloat16=parse_dtype(dtype) == torch.bfloat16, tied_dims=tied_dims)
         kernels = CudaKernels(device)
-    return Runtime(device=device, dtype=parse_dtype(dtype), kernels=kernels)
+    if weight_group is not None and not hasattr(kernels, "pack_weights"):
+        raise ValueError("these kernels have no matrices in 4 bits (weight_group)")
+    return Runtime(device=device, dtype=parse_dtype(dtype), kernels=kernels, weight_group=weight_group)
 
 
 def _align4(n: int) -> int:
@@ -116,9 +121,12 @@ class ModelRunner:
     # ------------------------------------------------------------ construction
     @classmethod
     def from_folder(cls, model_dir: str, dtype="bfloat16", device="cuda:0", page_size: int = 16,
-                    pool_tokens: int = 4096, max_requests: int = 4, kernels=None) -> "ModelRunner":
+                    pool_tokens: int = 4096, max_requests: int = 4, kernels=None,
+                    weight_group: Optional[int] = None) -> "ModelRunner":
+        """``weight_group``: None keeps the matrices as the checkpoint has them; 32, 64 or 128 puts those of attention and dense
+        feed-forwards and the output matrix into 4 bits while they are bound, with a scale for so many columns of a row."""
         _, _, spec = load_config(model_dir)
-        runtime = make_runtime(dtype, device, kernels, spec)
+        runtime = make_runtime(dtype, device, kernels, spec, weight_group)
         model = DecoderModel(spec, runtime)
         load_weights(model, model_dir, runtime)
         return cls(model, runtime, page_size, pool_tokens, max_requests)
@@ -126,7 +134,7 @@ class ModelRunner:
     @classmethod
     def from_random(cls, config_object: dict, seed: int = 0, dtype="bfloat16", device="cuda:0",
                     page_size: int = 16, pool_tokens: int = 4096, max_requests: int = 4,
-                    kernels=None, num_layers: Optional[int] = None) -> "ModelRunner":
+                    kernels=None, num_layers: Optional[int] = None, weight_group: Optional[int] = None) -> "ModelRunner":
         """A model of the architecture and sizes that ``config_object`` (the
         content of a config.json) names, with random weights made on the device.
         ``num_layers`` runs only the first layers (for measurements that must fit
@@ -137,7 +145,7 @@ class ModelRunner:
             config_object = dict(config_object, num_hidden_layers=num_layers)
         arch = find_architecture(config_object)
         spec = arch.model_spec(arch.read_config(config_object))
-        runtime = make_runtime(dtype, device, kernels, spec)
+        runtime = make_runtime(dtype, device, kernels, spec, weight_group)
         model = DecoderModel(spec, runtime)
         bind_random_weights(model, seed, runtime)
         return cls(model, runtime, page_size, pool_tokens, max_requests)

@@ -26,11 +26,20 @@ class PackedWeights:
 
     def __init__(self, data: torch.Tensor, rows: int, columns: int, group: int, paired: bool):
         self.data, self.rows, self.columns, self.group, self.paired = data, rows, columns, group, paired
+        self._parts = {}
         self.calls = {}              # (kernels, rows of x, types, activation) -> the arguments that stay the same
 
     @property
     def shape(self) -> torch.Size:
         return torch.Size((self.rows * (2 if self.paired else 1), self.columns))
+
+    def __getitem__(self, rows: slice) -> "PackedWeights":
+        """The matrix's first rows, ``w[:n]`` (no copy)."""
+        if self.paired or not isinstance(rows, slice) or rows.start is not None or rows.step is not None \
+                or not 0 < (self.rows if rows.stop is None else rows.stop) <= self.rows:
+            raise IndexError("the first rows of a matrix in 4 bits, w[:n], and nothing else")
+        n = self.rows if rows.stop is None else rows.stop
+        return self._parts.setdefault(n, PackedWeights(self.data, n, self.columns, self.group, False))
 
     @property
     def device(self) -> torch.device:

@@ -219,7 +219,8 @@ class PagedAttention(Mixer):
         if self.spec.distance_bias == "log":
             self.distance_r1 = tensors[self.names["distance_r1"]].float().contiguous()
             self.distance_r2 = tensors[self.names["distance_r2"]].float().contiguous()
-        self.o_proj = tensors[self.names["o_proj"]].contiguous()
+        self.qkv = self.runtime.pack(self.qkv)
+        self.o_proj = self.runtime.pack(tensors[self.names["o_proj"]].contiguous())
         if self.spec.qk_norm is not None:
             self.q_norm = tensors[self.names["q_norm"]].contiguous()
             self.k_norm = tensors[self.names["k_norm"]].to(self.q_norm.dtype).contiguous()
@@ -471,7 +472,7 @@ class PagedAttention(Mixer):
         takes = getattr(k, "finishes_heads", None)
         T = ctx.num_tokens
         nq, nkv, d = s.num_heads, s.num_kv_heads, s.head_dim
-        if takes is None or s.tied_values or not takes(T, d, fused[1], rt.dtype):
+        if takes is None or s.tied_values or rt.weight_group is not None or not takes(T, d, fused[1], rt.dtype):
             return False
         cos_sin = self.position.step_table(ctx)
         if cos_sin is None:

@@ -25,6 +25,11 @@ class Runtime:
     device: torch.device
     dtype: torch.dtype           # activations and caches: torch.bfloat16 or torch.float32
     kernels: object              # the operations (chibillm_b200.kernels.ops.CudaKernels)
+    weight_group: Optional[int] = None   # matrices in 4 bits with a scale for so many columns (None: as they are)
+
+    def pack(self, w: torch.Tensor):
+        """A matrix that only ``kernels.linear`` reads, in 4 bits if the run keeps its matrices so."""
+        return w if self.weight_group is None else self.kernels.pack_weights(w, self.weight_group)
 
     @property
     def is_float32(self) -> bool:

@@ -72,12 +72,16 @@ class GatedMLP(FeedForward):
             self.bias_gate_up = torch.cat([tensors[self.names["gate_bias"]].to(gate.dtype),
                                            tensors[self.names["up_bias"]].to(gate.dtype)]).contiguous()
             self.bias_down = tensors[self.names["down_bias"]].float().contiguous()
+        if self.runtime.weight_group is not None and self.fused_gate:
+            self.gate_up_interleaved = self.runtime.kernels.pack_gate_up(gate, up, self.runtime.weight_group)
+            self.down = self.runtime.pack(tensors[self.names["down_proj"]])
+            return
         interleave = getattr(self.runtime.kernels, "interleave_gate_up", None) if self.fused_gate else None
         self.gate_up_interleaved = interleave(gate, up) if interleave is not None else None
         # one of the two layouts is kept: blocks of 64 gate rows and their 64 up rows for the kernel
         # that applies SwiGLU itself, else gate rows followed by up rows
-        self.gate_up = None if self.gate_up_interleaved is not None else torch.cat([gate, up], dim=0).contiguous()
-        self.down = tensors[self.names["down_proj"]].contiguous()
+        self.gate_up = None if self.gate_up_interleaved is not None else self.runtime.pack(torch.cat([gate, up], dim=0).contiguous())
+        self.down = self.runtime.pack(tensors[self.names["down_proj"]].contiguous())
 
     accepts_scaled_rows = True       # x goes to the gate | up product and nowhere else
 
@@ -163,8 +167,8 @@ class DenseMLP(FeedForward):
         return out
 
     def bind(self, tensors: Dict[str, torch.Tensor]) -> None:
-        self.up = tensors[self.names["up_proj"]].contiguous()
-        self.down = tensors[self.names["down_proj"]].contiguous()
+        self.up = self.runtime.pack(tensors[self.names["up_proj"]].contiguous())
+        self.down = self.runtime.pack(tensors[self.names["down_proj"]].contiguous())
         if self.spec.biases:
             self.up_bias = tensors[self.names["up_bias"]].float().contiguous()
             self.output_bias = tensors[self.names["down_bias"]].float().contiguous()
