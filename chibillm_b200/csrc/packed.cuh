@@ -31,6 +31,7 @@ struct ChibiPackedCall {
     int splits, clusters, tokens;    // both kernels
     int warps, along_k, batch, depth, run;         // few rows
     int rounds;                      // many rows
+    unsigned long long map[16];      // the tensor map over the records (chibi_packed_prepare)
 };
 
 namespace chibi {

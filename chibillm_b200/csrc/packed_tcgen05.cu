@@ -22,6 +22,8 @@
 #include "split_f32.cuh"
 #include "tensor_map.cuh"
 
+#include <string.h>
+
 namespace chibi {
 namespace {
 
@@ -512,7 +514,7 @@ CHIBI_API int chibi_packed_many_rows(const ChibiPackedCall* c, const void* x, lo
         return CHIBI_ERR_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(x) & 15) || x_stride % 8)
         return CHIBI_ERR_UNSUPPORTED;
-    const int each = c->pair ? PACKED_ROWS / 2 : PACKED_ROWS, tile_rows = c->pair ? PT_ROWS / 2 : PT_ROWS;
+    const int tile_rows = c->pair ? PT_ROWS / 2 : PT_ROWS;
     const long long token_tiles = (c->m + (long long)tokens - 1) / tokens, tiles = (c->n + (long long)tile_rows - 1) / tile_rows * token_tiles;
     if (tiles > 0x3fffffff)
         return CHIBI_ERR_UNSUPPORTED;
@@ -520,9 +522,9 @@ CHIBI_API int chibi_packed_many_rows(const ChibiPackedCall* c, const void* x, lo
     if (splits > 1 ? tiles < whole || tiles - whole > c->clusters : tiles > whole)
         return CHIBI_ERR_ARGUMENT;             // the pieces are not all tiles, each once
     CUtensorMap map_w, map;
-    if (!packed_map(c->data, c->group, (c->n + each - 1) / each, chunks, 1, PT_ROWS / PACKED_ROWS, &map_w)
-        || !tensor_map_2d(x, c->m, c->k, x_stride, tokens, &map))
+    if (!tensor_map_2d(x, c->m, c->k, x_stride, tokens, &map))
         return CHIBI_ERR_UNSUPPORTED;
+    memcpy(&map_w, c->map, sizeof(map_w));
     const PackedProduct p { chunks, c->n, c->pair, c->m, out, c->out_type, out_stride, (const float*)residual, residual_stride, c->act,
                             c->rounds, splits, (int)tiles, (int)token_tiles, (int*)c->error };
     const int ctas = c->clusters * splits;

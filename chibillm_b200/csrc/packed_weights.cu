@@ -5,6 +5,7 @@
 #include "sm100.cuh"
 
 #include <cuda_fp16.h>
+#include <string.h>
 
 #include <type_traits>
 
@@ -16,8 +17,10 @@ namespace {
 // 16 neighbouring lanes) find its largest element together.
 //   s = bf16(m / -8), m the element of largest magnitude, the first of equals; q = w / s rounded to nearest, ties to even,
 //   within -8 ... 7.  A group with what is not a finite number has the scale NaN.
-// w / s is rounded to 32 bits before it is rounded to a whole number, which may go wrong next to a half; w - q s is exact
-// (q s has 12 bits, and the difference no more than w has), so it is compared with s / 2.
+// The quotient is w times 1 / s and one correction from what is left of w (exact), which makes it the 32-bit number nearest to
+// w / s.  For bfloat16 w that decides: w / s has 8 bits over 8 bits, so it is a half or far from one.  A 32-bit w / s can be so close
+// to a half that the nearest 32-bit number is the half itself; a thread that meets one decides again with w - q s, which is exact
+// (q s has 12 bits, and the difference no more than w has).
 struct PackSource {
     const void* w[2];          // a matrix, or gate and up
     long long stride[2];
@@ -25,14 +28,56 @@ struct PackSource {
     int pair;
 };
 
-__device__ __forceinline__ int nearest_code(float w, float s)
+// q + 8 for an element next to a half, by w - q s against s / 2.
+__device__ __noinline__ uint32_t code_next_to_a_half(float w, float s)
 {
     float q = fminf(fmaxf(rintf(w / s), -9.f), 8.f);
     const float rest = fmaf(-q, s, w), half = 0.5f * fabsf(s);
     const float away = (rest > 0.f) == (s > 0.f) ? 1.f : -1.f;
     if (fabsf(rest) > half || (fabsf(rest) == half && ((int)q & 1)))
         q += away;
-    return (int)fminf(fmaxf(q, -8.f), 7.f);
+    return (uint32_t)((int)fminf(fmaxf(q, -8.f), 7.f) + 8);
+}
+
+template <typename T> __device__ __forceinline__ uint32_t code_word(const float (&v)[8], float s)
+{
+    // (1.5 2^23 + 8: the sum's last bits are the whole number plus 8)
+    constexpr float SHIFT = 12582920.f;
+    const float by = 1.f / s;
+    uint32_t word = 0;
+    float far = 0.f;                             // the largest distance from a whole number
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float t = v[i] * by;
+        const float q = fminf(fmaxf(fmaf(fmaf(-t, s, v[i]), by, t), -8.f), 7.f);
+        const float sum = q + SHIFT;
+        if (sizeof(T) == 4)
+            far = fmaxf(far, fabsf(q - (sum - SHIFT)));
+        word |= (__float_as_uint(sum) & 15u) << (4 * (i / 2) + 16 * (i & 1));
+    }
+    // (1 / s of the smallest s is infinite)
+    if (far < 0.5f && fabsf(by) < INFINITY)
+        return word;
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        word |= code_next_to_a_half(v[i], s) << (4 * (i / 2) + 16 * (i & 1));
+    return word;
+}
+
+// 8 neighbouring numbers of a row from column `col` on, zeros beyond its k columns.
+template <typename T> __device__ __forceinline__ void read_eight(const T* row, int col, int k, T (&v)[8])
+{
+    const T* src = row + col;
+    if (col + 8 <= k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = col + i < k ? src[i] : from_f32<T>(0.f);
+    }
 }
 
 template <typename T>
@@ -43,25 +88,24 @@ __global__ void __launch_bounds__(512) pack_kernel(PackSource p, int row_blocks,
     pdl_wait();
     const int r = threadIdx.x >> 4, seg = threadIdx.x & 15;
     const int lanes = group / 8;
-    for (long long record = blockIdx.x; record < (long long)row_blocks * col_blocks; record += gridDim.x) {
-        const int rb = (int)(record / col_blocks), cb = (int)(record % col_blocks);
+    const int records = row_blocks * col_blocks;
+    auto fetch = [&](int record, T (&raw)[8]) {
+        const int rb = record / col_blocks, cb = record - rb * col_blocks;
         const int side = packed_side(p.pair, r), row = packed_source_row(p.pair, rb, r);
-        const int col = cb * PACKED_COLS + seg * 8;
+        // (a row beyond the matrix is read as one without columns)
+        read_eight(static_cast<const T*>(p.w[side]) + (row < p.rows ? (long long)row * p.stride[side] : 0), cb * PACKED_COLS + seg * 8,
+                   row < p.rows ? p.cols : 0, raw);
+    };
+    T raw[8];
+    if ((int)blockIdx.x < records)
+        fetch(blockIdx.x, raw);
+    for (int record = blockIdx.x; record < records; record += gridDim.x) {
         float v[8];
-        const T* src = static_cast<const T*>(p.w[side]) + (long long)row * p.stride[side] + col;
-        if (row < p.rows && col + 8 <= p.cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-            T raw[8];
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-                reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(src)[i];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = to_f32(raw[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = row < p.rows && col + i < p.cols ? to_f32(src[i]) : 0.f;
-        }
+        for (int i = 0; i < 8; ++i)
+            v[i] = to_f32(raw[i]);
+        if (record + (int)gridDim.x < records)
+            fetch(record + gridDim.x, raw);          // the next one is on its way meanwhile
         // the first element of largest magnitude; what is not finite counts as larger than everything
         float best = v[0];
         bool finite = isfinite(v[0]);
@@ -81,14 +125,8 @@ __global__ void __launch_bounds__(512) pack_kernel(PackSource p, int row_blocks,
         const float s = __bfloat162float(s16);
         if (s == 0.f)
             s16 = __float2bfloat16_rn(0.f);      // (no minus zeros)
-        uint32_t word = 0x88888888u;
-        if (finite && s != 0.f) {
-            word = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                word |= (uint32_t)(nearest_code(v[i], s) + 8) << (4 * (i / 2) + 16 * (i & 1));
-        }
-        uint8_t* dst = out + record * packed_record_bytes(group);
+        const uint32_t word = finite && s != 0.f ? code_word<T>(v, s) : 0x88888888u;
+        uint8_t* dst = out + (long long)record * packed_record_bytes(group);
         *reinterpret_cast<uint32_t*>(dst + packed_word_at(r, seg)) = word;
         if (seg % lanes == 0)
             *reinterpret_cast<__nv_bfloat16*>(dst + packed_scale_at(r, seg / lanes)) = s16;
@@ -108,8 +146,8 @@ __global__ void __launch_bounds__(512) pack_codes_kernel(CodeSource p, int row_b
     pdl_wait();
     const int r = threadIdx.x >> 4, seg = threadIdx.x & 15;
     const int lanes = group / 8;
-    for (long long record = blockIdx.x; record < (long long)row_blocks * col_blocks; record += gridDim.x) {
-        const int rb = (int)(record / col_blocks), cb = (int)(record % col_blocks);
+    for (int record = blockIdx.x; record < row_blocks * col_blocks; record += gridDim.x) {
+        const int rb = record / col_blocks, cb = record % col_blocks;
         const int side = packed_side(p.pair, r), row = packed_source_row(p.pair, rb, r);
         const int col = cb * PACKED_COLS + seg * 8;
         uint32_t word = 0;
@@ -118,7 +156,7 @@ __global__ void __launch_bounds__(512) pack_codes_kernel(CodeSource p, int row_b
             const int q = row < p.rows && col + i < p.cols ? p.codes[side][(long long)row * p.stride[side] + col + i] : 0;
             word |= (uint32_t)((q + 8) & 15) << (4 * (i / 2) + 16 * (i & 1));
         }
-        uint8_t* dst = out + record * packed_record_bytes(group);
+        uint8_t* dst = out + (long long)record * packed_record_bytes(group);
         *reinterpret_cast<uint32_t*>(dst + packed_word_at(r, seg)) = word;
         if (seg % lanes == 0)
             *reinterpret_cast<__nv_bfloat16*>(dst + packed_scale_at(r, seg / lanes))
@@ -132,28 +170,31 @@ __global__ void __launch_bounds__(512) unpack_kernel(const uint8_t* data, int ro
                                                      int pair, T* out, long long stride)
 {
     pdl_enter();
-    const int r = threadIdx.x >> 4, seg = threadIdx.x & 15;
-    for (long long record = blockIdx.x; record < (long long)row_blocks * col_blocks; record += gridDim.x) {
-        const int rb = (int)(record / col_blocks), cb = (int)(record % col_blocks);
-        const int row = packed_source_row(pair, rb, r);
-        const int col = cb * PACKED_COLS + seg * 8;
-        if (row >= rows || col >= cols)
-            continue;
-        const uint8_t* src = data + record * packed_record_bytes(group);
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(src + packed_word_at(r, seg));
-        const float s = to_f32(*reinterpret_cast<const __nv_bfloat16*>(src + packed_scale_at(r, seg * 8 / group)));
-        T* dst = out + (long long)(row + packed_side(pair, r) * rows) * stride + col;
-        T v[8];
+    // 16 bytes of the output a thread, neighbours side by side
+    constexpr int EACH = 16 / sizeof(T), ROW_THREADS = PACKED_COLS / EACH;
+    for (int record = blockIdx.x; record < row_blocks * col_blocks; record += gridDim.x) {
+        const int rb = record / col_blocks, cb = record - rb * col_blocks;
+        const uint8_t* src = data + (long long)record * packed_record_bytes(group);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = from_f32<T>((float)((int)((word >> (4 * (i / 2) + 16 * (i & 1))) & 15) - 8) * s);
-        if (col + 8 <= cols && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+        for (int i = threadIdx.x; i < PACKED_ROWS * ROW_THREADS; i += 512) {
+            const int r = i / ROW_THREADS, at = i % ROW_THREADS * EACH;
+            const int row = packed_source_row(pair, rb, r), col = cb * PACKED_COLS + at;
+            if (row >= rows || col >= cols)
+                continue;
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(src + packed_word_at(r, at >> 3));
+            const float s = to_f32(*reinterpret_cast<const __nv_bfloat16*>(src + packed_scale_at(r, at / group)));
+            T* dst = out + (long long)(row + packed_side(pair, r) * rows) * stride + col;
+            T v[EACH];
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-                reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
-        } else {
-            for (int i = 0; i < 8 && col + i < cols; ++i)
-                dst[i] = v[i];
+            for (int j = 0; j < EACH; ++j) {
+                const int e = (at & 7) + j;
+                v[j] = from_f32<T>((float)((int)((word >> (4 * (e / 2) + 16 * (e & 1))) & 15) - 8) * s);
+            }
+            if (col + EACH <= cols && (reinterpret_cast<uintptr_t>(dst) & 15) == 0)
+                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+            else
+                for (int j = 0; j < EACH && col + j < cols; ++j)
+                    dst[j] = v[j];
         }
     }
 }
@@ -216,21 +257,6 @@ __device__ __forceinline__ float peer_shared_f32(uint32_t own_smem_addr, uint32_
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sm100::peer_smem_addr(own_smem_addr, rank)) : "memory");
     return v;
-}
-
-// 8 neighbouring numbers of a row of x from column `col` on, zeros beyond its k columns.
-template <typename T> __device__ __forceinline__ void read_eight(const T* row, int col, int k, T (&v)[8])
-{
-    const T* src = row + col;
-    if (col + 8 <= k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-            reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = col + i < k ? src[i] : from_f32<T>(0.f);
-    }
 }
 
 // The exponent of the power of two by which a row is multiplied, from its largest finite magnitude: none where that is
@@ -551,6 +577,13 @@ void (*few_rows_kernel(bool x32, int tokens, int group))(const CUtensorMap, cons
                : (tokens <= 8 ? few_rows_kernel_of<1, false>(group) : few_rows_kernel_of<2, false>(group));
 }
 
+// Four blocks to an SM, which go over the records together.
+dim3 pack_grid(long long records)
+{
+    const long long most = 4LL * device_sm_count();
+    return dim3((unsigned)(records < most ? records : most));
+}
+
 } // namespace
 } // namespace chibi
 
@@ -566,7 +599,9 @@ CHIBI_API int chibi_pack_weights(const void* w, const void* up, int type, int ro
     const int each = up ? PACKED_ROWS / 2 : PACKED_ROWS;
     const int row_blocks = (rows + each - 1) / each, col_blocks = (cols + PACKED_COLS - 1) / PACKED_COLS;
     const long long records = (long long)row_blocks * col_blocks;
-    CHIBI_DISPATCH_TYPE(type, T, launch(pack_kernel<T>, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(512), 0,
+    if (records > 0x3fffffff)
+        return CHIBI_ERR_UNSUPPORTED;
+    CHIBI_DISPATCH_TYPE(type, T, launch(pack_kernel<T>, pack_grid(records), dim3(512), 0,
                                         (cudaStream_t)stream, src, row_blocks, col_blocks, group, (uint8_t*)out));
     return launch_status();
 }
@@ -583,7 +618,9 @@ CHIBI_API int chibi_pack_codes(const void* codes, const void* scales, const void
     const int each = up_codes ? PACKED_ROWS / 2 : PACKED_ROWS;
     const int row_blocks = (rows + each - 1) / each, col_blocks = (cols + PACKED_COLS - 1) / PACKED_COLS;
     const long long records = (long long)row_blocks * col_blocks;
-    launch(pack_codes_kernel, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(512), 0, (cudaStream_t)stream, src, row_blocks,
+    if (records > 0x3fffffff)
+        return CHIBI_ERR_UNSUPPORTED;
+    launch(pack_codes_kernel, pack_grid(records), dim3(512), 0, (cudaStream_t)stream, src, row_blocks,
            col_blocks, group, (uint8_t*)out);
     return launch_status();
 }
@@ -596,7 +633,9 @@ CHIBI_API int chibi_unpack_weights(const void* data, int rows, int cols, int pai
     const int each = pair ? PACKED_ROWS / 2 : PACKED_ROWS;
     const int row_blocks = (rows + each - 1) / each, col_blocks = (cols + PACKED_COLS - 1) / PACKED_COLS;
     const long long records = (long long)row_blocks * col_blocks;
-    CHIBI_DISPATCH_TYPE(out_type, T, launch(unpack_kernel<T>, dim3((unsigned)(records < 65536 ? records : 65536)), dim3(512), 0,
+    if (records > 0x3fffffff)
+        return CHIBI_ERR_UNSUPPORTED;
+    CHIBI_DISPATCH_TYPE(out_type, T, launch(unpack_kernel<T>, pack_grid(records), dim3(512), 0,
                                             (cudaStream_t)stream, (const uint8_t*)data, row_blocks, col_blocks, group, rows, cols, pair,
                                             (T*)out, stride));
     return launch_status();
@@ -634,6 +673,21 @@ CHIBI_API int chibi_packed_few_rows_clusters(int x32, int group, int tokens, int
     return clusters;
 }
 
+// Fills in what a call keeps beside its sizes: the tensor map over the records.  `many`: for chibi_packed_many_rows.
+CHIBI_API int chibi_packed_prepare(ChibiPackedCall* c, int many)
+{
+    if (!c || !c->data || c->n < 1 || c->k < 1 || !packed_group_ok(c->group) || (!many && (c->run < 1 || c->run > 256)))
+        return CHIBI_ERR_ARGUMENT;
+    const int each = c->pair ? PACKED_ROWS / 2 : PACKED_ROWS;
+    CUtensorMap map;
+    if (!packed_map(c->data, c->group, (c->n + each - 1) / each, (c->k + PACKED_COLS - 1) / PACKED_COLS, many ? 1 : c->run,
+                    many ? 128 / PACKED_ROWS : 1, &map))
+        return CHIBI_ERR_UNSUPPORTED;
+    static_assert(sizeof(map) == sizeof(c->map), "");
+    memcpy(c->map, &map, sizeof(map));
+    return CHIBI_OK;
+}
+
 // out[m, n] = x[m, k] times the matrix (+ residual); pair: act(x gate) * (x up), n features.  The plan: see FewRows.
 CHIBI_API int chibi_packed_few_rows(const ChibiPackedCall* c, const void* x, long long x_stride, void* out, long long out_stride,
                                     const void* residual, long long residual_stride, void* stream)
@@ -651,9 +705,10 @@ CHIBI_API int chibi_packed_few_rows(const ChibiPackedCall* c, const void* x, lon
     const size_t smem = few_rows_smem(x32, c->group, chunks, c->warps, c->splits, c->batch, c->depth, c->run, c->tokens);
     const long long token_blocks = ((long long)c->m + c->tokens - 1) / c->tokens;
     const int each = c->pair ? PACKED_ROWS / 2 : PACKED_ROWS, row_blocks = (c->n + each - 1) / each;
-    CUtensorMap map;
-    if (smem > FEW_SMEM_LIMIT || token_blocks > 65535 || !packed_map(c->data, c->group, row_blocks, chunks, c->run, 1, &map))
+    if (smem > FEW_SMEM_LIMIT || token_blocks > 65535)
         return CHIBI_ERR_UNSUPPORTED;
+    CUtensorMap map;
+    memcpy(&map, c->map, sizeof(map));
     const FewRows p { row_blocks, chunks, c->n, c->k, c->pair, x, x_stride, c->m, out, c->out_type, out_stride, (const float*)residual,
                       residual_stride, c->act, c->warps, c->splits, c->along_k, c->batch, c->depth, c->run, c->tokens, c->clusters,
                       (int*)c->error };

@@ -106,6 +106,7 @@ _SIGNATURES = {
         "chibi_pack_weights": [P, P, I, I, I, L, L, I, P, P],
         "chibi_pack_codes": [P, P, P, P, I, I, L, L, L, L, I, P, P],
         "chibi_unpack_weights": [P, I, I, I, I, P, I, L, P],
+        "chibi_packed_prepare": [P, I],
         "chibi_packed_many_rows": [P, P, L, P, L, P, L, P],
         "chibi_packed_many_rows_clusters": [I],
         "chibi_packed_few_rows_kb": [I, I, I, I, I, I, I, I, I],
@@ -147,7 +148,7 @@ class PackedCall(ctypes.Structure):
     """ChibiPackedCall of packed.cuh: what stays the same from call to call of a product with a matrix in 4 bits."""
     _fields_ = [("data", c_void_p), ("error", c_void_p)] + [(name, c_int) for name in (
         "group", "n", "k", "pair", "m", "x_type", "out_type", "act", "splits", "clusters", "tokens", "warps", "along_k", "batch", "depth",
-        "run", "rounds")]
+        "run", "rounds")] + [("map", ctypes.c_ulonglong * 16)]
 
 
 class HeadsOut(ctypes.Structure):

@@ -139,6 +139,11 @@ class DeferredProduct:
 
 _STREAM_SCRATCH: Dict[torch.device, torch.Tensor] = {}
 
+# what the device says about clusters of the products with matrices in 4 bits, and how their work is shared out, by sizes
+_PACKED_CLUSTERS: Dict[tuple, int] = {}
+_PACKED_PLANS: Dict[int, Dict[tuple, FewRowsPlan]] = {}
+_PACKED_CUTS: Dict[int, Dict[tuple, ManyRowsCut]] = {}
+
 # torch's own fast path to the current stream's handle (a plain integer): the public
 # torch.cuda.current_stream() builds a Stream object through several Python layers, a quarter
 # of the host time of a step that launches a few hundred kernels
@@ -181,9 +186,9 @@ class CudaKernels:
         self.use_tcgen05_attention = True
         # matrices in 4 bits: up to so many bfloat16 rows of x stream the matrix once through mma.sync, more go to tcgen05
         self.packed_few_rows_max = 12
-        self._packed_plans: Dict[tuple, FewRowsPlan] = {}
-        self._packed_cuts: Dict[tuple, ManyRowsCut] = {}
-        self._packed_clusters: Optional[list] = None
+        # (by sizes, for all kernels of a process on this device)
+        self._packed_plans: Dict[tuple, FewRowsPlan] = _PACKED_PLANS.setdefault(self._device_index, {})
+        self._packed_cuts: Dict[tuple, ManyRowsCut] = _PACKED_CUTS.setdefault(self._device_index, {})
         self._partial_bufs = [None, None]
         self._partial_turn = 0
         self._partial_stamps = [0, 0]     # how often each of the two arrays has been handed out
@@ -877,9 +882,16 @@ class CudaKernels:
         plan = self._packed_plans.get(key)
         if plan is None:
             lib, x = self.lib, int(x32)
+
+            def most_clusters(tokens, warps, splits, kb):
+                # (an instantiation takes up to 8 tokens, or up to 16)
+                asked = (self._device_index, x, w.group, tokens <= 8, warps, splits, kb)
+                if asked not in _PACKED_CLUSTERS:
+                    _PACKED_CLUSTERS[asked] = lib.chibi_packed_few_rows_clusters(x, w.group, tokens, warps, splits, kb)
+                return _PACKED_CLUSTERS[asked]
+
             plan = few_rows_plan(w.rows, w.columns, w.paired, m, x32,
-                                 lambda *cut: lib.chibi_packed_few_rows_kb(x, w.group, w.columns, *cut),
-                                 lambda *cut: lib.chibi_packed_few_rows_clusters(x, w.group, *cut), self.sm_count)
+                                 lambda *cut: lib.chibi_packed_few_rows_kb(x, w.group, w.columns, *cut), most_clusters, self.sm_count)
             if plan is None:
                 raise KernelError(f"a product over {w.columns} columns in 4 bits: more than the kernel holds")
             if len(self._packed_plans) > 4096:
@@ -892,9 +904,13 @@ class CudaKernels:
         key = (w.rows, w.columns, w.paired, m)
         cut = self._packed_cuts.get(key)
         if cut is None:
-            if self._packed_clusters is None:
-                self._packed_clusters = [0] + [self.lib.chibi_packed_many_rows_clusters(s) for s in range(1, 9)]
-            cut = many_rows_cut(w.rows, w.columns, w.paired, m, lambda splits: self._packed_clusters[splits])
+            def most_clusters(splits):
+                asked = (self._device_index, splits)
+                if asked not in _PACKED_CLUSTERS:
+                    _PACKED_CLUSTERS[asked] = self.lib.chibi_packed_many_rows_clusters(splits)
+                return _PACKED_CLUSTERS[asked]
+
+            cut = many_rows_cut(w.rows, w.columns, w.paired, m, most_clusters)
             if len(self._packed_cuts) > 4096:
                 self._packed_cuts.clear()
             self._packed_cuts[key] = cut
@@ -906,7 +922,9 @@ class CudaKernels:
                                   self.ACTIVATIONS[kind] if kind else 0)
         for name, value in (self.packed_cut(w, m) if many else self.packed_plan(w, m, x_code == F32))._asdict().items():
             setattr(call, name, value)
-        return ctypes.pointer(call)
+        pointer = ctypes.pointer(call)
+        _check(self.lib.chibi_packed_prepare(pointer, int(many)), "a product with a matrix in 4 bits")
+        return pointer
 
     def _packed_product(self, x, w: PackedWeights, out: torch.Tensor, residual: Optional[torch.Tensor], kind: Optional[str],
                         what: str) -> None:
@@ -915,13 +933,15 @@ class CudaKernels:
         if w.paired != (kind is not None):
             raise KernelError(f"{what}: a pair of matrices (pack_gate_up) belongs to linear_swiglu, any other to linear")
         self._on_this_device(what, x, w.data, out, residual)
-        _rows_contiguous(x, what)
-        _rows_contiguous(out, what)
+        x_strides, out_strides = x.stride(), out.stride()
+        if len(x_strides) != 2 or x_strides[1] != 1 or len(out_strides) != 2 or out_strides[1] != 1:
+            _rows_contiguous(x, f"{what}: x")
+            _rows_contiguous(out, f"{what}: out")
         M, K = x.shape
         if K != w.columns or out.shape != (M, w.rows):
             raise KernelError(f"{what}: shapes x {tuple(x.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
         if residual is not None:
-            _rows_contiguous(residual, what)
+            _rows_contiguous(residual, f"{what}: residual")
             if residual.dtype != torch.float32 or residual.shape != out.shape:
                 raise KernelError(f"{what}: residual must be float32 [M, N]")
         x_code, out_code = _code(x), _code(out)
@@ -930,8 +950,8 @@ class CudaKernels:
         if torch.cuda.current_device() != self._device_index:
             with torch.cuda.device(self._device_index):
                 return self._packed_product(x, w, out, residual, kind, what)
-        rest = (_ptr(x), x.stride(0), _ptr(out), out.stride(0), _ptr(residual), residual.stride(0) if residual is not None else 0,
-                self._stream())
+        rest = (x.data_ptr(), x_strides[0], out.data_ptr(), out_strides[0], None if residual is None else residual.data_ptr(),
+                0 if residual is None else residual.stride(0), self._stream())
         for many in ((True, False) if x_code == BF16 and M > self.packed_few_rows_max else (False,)):
             key = (self, w.data.data_ptr(), M, x_code, out_code, kind, many)
             call = w.calls.get(key)
