@@ -25,6 +25,10 @@ class KernelError(RuntimeError):
     pass
 
 
+# torch's own fast path to the current device's index
+_raw_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _code(t: torch.Tensor) -> int:
     try:
         return _CODES[t.dtype]
@@ -916,56 +920,65 @@ class CudaKernels:
             self._packed_cuts[key] = cut
         return cut
 
-    def _packed_call(self, w: PackedWeights, m: int, x_code: int, out_code: int, kind: Optional[str], many: bool):
-        """The arguments of a product that stay the same from call to call."""
-        call = library.PackedCall(_ptr(w.data), _ptr(self.error), w.group, w.rows, w.columns, int(w.paired), m, x_code, out_code,
-                                  self.ACTIVATIONS[kind] if kind else 0)
-        for name, value in (self.packed_cut(w, m) if many else self.packed_plan(w, m, x_code == F32))._asdict().items():
-            setattr(call, name, value)
-        pointer = ctypes.pointer(call)
-        _check(self.lib.chibi_packed_prepare(pointer, int(many)), "a product with a matrix in 4 bits")
-        return pointer
-
-    def _packed_product(self, x, w: PackedWeights, out: torch.Tensor, residual: Optional[torch.Tensor], kind: Optional[str],
-                        what: str) -> None:
-        if isinstance(x, ScaledRows):
-            x = x.materialise()
+    def _packed_call(self, x: torch.Tensor, w: PackedWeights, out: torch.Tensor, kind: Optional[str], many: bool, what: str):
+        """What stays the same from call to call of a product: its arguments, made once for the sizes and types of x and out.
+        (entry point, arguments, out's shape, whether the kernel may refuse x's strides)"""
         if w.paired != (kind is not None):
             raise KernelError(f"{what}: a pair of matrices (pack_gate_up) belongs to linear_swiglu, any other to linear")
-        self._on_this_device(what, x, w.data, out, residual)
+        _rows_contiguous(x, f"{what}: x")
+        if x.shape[1] != w.columns:
+            raise KernelError(f"{what}: shapes x {tuple(x.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
+        m, x_code = x.shape[0], _code(x)
+        call = library.PackedCall(_ptr(w.data), _ptr(self.error), w.group, w.rows, w.columns, int(w.paired), m, x_code, _code(out),
+                                  self.ACTIVATIONS[kind] if kind else 0)
+        many = many and x_code == BF16 and m > self.packed_few_rows_max
+        if m > 0:
+            for name, value in (self.packed_cut(w, m) if many else self.packed_plan(w, m, x_code == F32))._asdict().items():
+                setattr(call, name, value)
+        pointer = ctypes.pointer(call)
+        if m > 0:
+            _check(self.lib.chibi_packed_prepare(pointer, int(many)), what)
+        return self.lib.chibi_packed_many_rows if many else self.lib.chibi_packed_few_rows, pointer, torch.Size((m, w.rows)), many
+
+    def _packed_product(self, x, w: PackedWeights, out: torch.Tensor, residual: Optional[torch.Tensor], kind: Optional[str],
+                        what: str, many: bool = True) -> None:
+        if isinstance(x, ScaledRows):
+            x = x.materialise()
+        here, data = self._device_index, w.data
+        if x.get_device() != here or out.get_device() != here or data.get_device() != here \
+                or (residual is not None and residual.get_device() != here):
+            self._on_this_device(what, x, data, out, residual)
+        if _raw_current_device() != here:
+            with torch.cuda.device(here):
+                return self._packed_product(x, w, out, residual, kind, what, many)
+        key = (self, self.lib, self.packed_few_rows_max, data.data_ptr(), x.shape, x.dtype, out.dtype, kind, many)
+        made = w.calls.get(key)
+        if made is None:
+            made = self._packed_call(x, w, out, kind, many, what)
+            if len(w.calls) > 256:
+                w.calls.clear()
+            w.calls[key] = made
+        entry, call, out_shape, may_refuse = made
         x_strides, out_strides = x.stride(), out.stride()
-        if len(x_strides) != 2 or x_strides[1] != 1 or len(out_strides) != 2 or out_strides[1] != 1:
+        if out.shape != out_shape:
+            raise KernelError(f"{what}: shapes x {tuple(x.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
+        if x_strides[1] != 1 or out_strides[1] != 1:
             _rows_contiguous(x, f"{what}: x")
             _rows_contiguous(out, f"{what}: out")
-        M, K = x.shape
-        if K != w.columns or out.shape != (M, w.rows):
-            raise KernelError(f"{what}: shapes x {tuple(x.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
+        residual_at = residual_stride = 0
         if residual is not None:
             _rows_contiguous(residual, f"{what}: residual")
-            if residual.dtype != torch.float32 or residual.shape != out.shape:
+            if residual.dtype != torch.float32 or residual.shape != out_shape:
                 raise KernelError(f"{what}: residual must be float32 [M, N]")
-        x_code, out_code = _code(x), _code(out)
-        if M == 0:
+            residual_at, residual_stride = residual.data_ptr(), residual.stride(0)
+        if out_shape[0] == 0:
             return
-        if torch.cuda.current_device() != self._device_index:
-            with torch.cuda.device(self._device_index):
-                return self._packed_product(x, w, out, residual, kind, what)
-        rest = (x.data_ptr(), x_strides[0], out.data_ptr(), out_strides[0], None if residual is None else residual.data_ptr(),
-                0 if residual is None else residual.stride(0), self._stream())
-        for many in ((True, False) if x_code == BF16 and M > self.packed_few_rows_max else (False,)):
-            key = (self, w.data.data_ptr(), M, x_code, out_code, kind, many)
-            call = w.calls.get(key)
-            if call is None:
-                if len(w.calls) > 256:
-                    w.calls.clear()
-                call = w.calls[key] = self._packed_call(w, M, x_code, out_code, kind, many)
-            status = (self.lib.chibi_packed_many_rows if many else self.lib.chibi_packed_few_rows)(call, *rest)
-            if many and status == -2:
-                continue                 # rows of x that a tile copy cannot fetch
-            _check(status, what)
-            self.launches += 1
-            self.tensor_core_calls += 1
-            return
+        status = entry(call, x.data_ptr(), x_strides[0], out.data_ptr(), out_strides[0], residual_at, residual_stride, self._stream())
+        if status == -2 and may_refuse:          # rows of x that a tile copy cannot fetch
+            return self._packed_product(x, w, out, residual, kind, what, many=False)
+        _check(status, what)
+        self.launches += 1
+        self.tensor_core_calls += 1
 
     def qk_norm_rope_append(self, qkv: torch.Tensor, q_out: torch.Tensor,
                             k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
