@@ -85,6 +85,14 @@ template <typename T> __device__ __forceinline__ void read_eight(const T* row, i
     }
 }
 
+// Products fetch their matrix before the kernel ahead of them has ended.  So the kernels that write one let nothing start early
+// (no pdl_trigger; and no mark in a timeline), and every thread's stores are performed, for tile copies too, before it ends.
+__device__ __forceinline__ void packed_done()
+{
+    __threadfence();
+    asm volatile("fence.proxy.async;" ::: "memory");
+}
+
 // A block's records, gridDim.x apart.
 struct RecordWalk {
     int rb, cb, rows_step, cols_step, col_blocks;
@@ -107,9 +115,7 @@ struct RecordWalk {
 template <typename T>
 __global__ void __launch_bounds__(128, 8) pack_kernel(PackSource p, int row_blocks, int col_blocks, int group, uint8_t* out)
 {
-    // (No pdl_trigger: products read their matrix before the kernel ahead of them has ended, so nothing may start before
-    // this kernel has.)
-    pdl_wait();
+    pdl_wait_now();                                  // (see packed_done)
     const int r = threadIdx.x >> 2, b = threadIdx.x & 3;
     const int lanes = group / 32;
     const int side = packed_side(p.pair, r);
@@ -179,6 +185,7 @@ __global__ void __launch_bounds__(128, 8) pack_kernel(PackSource p, int row_bloc
         if (b % lanes == 0)
             *reinterpret_cast<__nv_bfloat16*>(dst + packed_scale_at(r, b / lanes)) = s16;
     }
+    packed_done();
 }
 
 // Whole numbers and scales that somebody else has made, into records.
@@ -191,7 +198,7 @@ struct CodeSource {
 
 __global__ void __launch_bounds__(512, 4) pack_codes_kernel(CodeSource p, int row_blocks, int col_blocks, int group, uint8_t* out)
 {
-    pdl_wait();
+    pdl_wait_now();
     const int r = threadIdx.x >> 4, seg = threadIdx.x & 15;
     const int lanes = group / 8;
     for (RecordWalk at(col_blocks); at.rb < row_blocks; at.next()) {
@@ -210,6 +217,7 @@ __global__ void __launch_bounds__(512, 4) pack_codes_kernel(CodeSource p, int ro
             *reinterpret_cast<__nv_bfloat16*>(dst + packed_scale_at(r, seg / lanes))
                 = row < p.rows && col < p.cols ? p.scales[side][(long long)row * p.scale_stride[side] + col / group] : __float2bfloat16_rn(0.f);
     }
+    packed_done();
 }
 
 // The values, rows of a pair's first matrix before those of its second.  A thread makes 16 neighbouring bytes of the output, so a
@@ -302,8 +310,8 @@ struct FewRows {
     const float* residual;
     long long residual_stride;
     int act;                       // pairs: 1 gelu with tanh, 2 silu
-    int warps, splits, along_k, batch, depth, run, tokens;     // run: records of a stage; tokens: rows of x of a CTA
-    int clusters;
+    int warps, split_shift, along_shift, batch, depth, run, tokens;  // run: records of a stage; tokens: rows of x of a CTA
+    int clusters, units;
     int* error;
 };
 
@@ -358,14 +366,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     extern __shared__ __align__(1024) uint8_t smem[];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = p.splits > 1 ? (int)cluster_cta_rank() : 0;
-    const int cluster = blockIdx.x / p.splits;
+    const int splits = 1 << p.split_shift, along_k = 1 << p.along_shift;
+    if (threadIdx.x == 0)
+        tma_prefetch_descriptor(&map);
+    const int rank = splits > 1 ? (int)cluster_cta_rank() : 0;
+    const int cluster = blockIdx.x >> p.split_shift;
     const int token0 = blockIdx.y * p.tokens;
     const int tokens = min(p.tokens, p.m - token0);
-    const int c0 = (int)((long long)p.chunks * rank / p.splits), c1 = (int)((long long)p.chunks * (rank + 1) / p.splits);
-    const int most = (p.chunks + p.splits - 1) / p.splits;
-    const int blocks_per_unit = p.warps / p.along_k;
-    const int units = (p.row_blocks + blocks_per_unit - 1) / blocks_per_unit;
+    const int c0 = (p.chunks * rank) >> p.split_shift, c1 = (p.chunks * (rank + 1)) >> p.split_shift;
+    const int most = (p.chunks + splits - 1) >> p.split_shift;
+    const int unit_shift = (p.warps == 16 ? 4 : 3) - p.along_shift, blocks_per_unit = 1 << unit_shift;
 
     // shared memory: rings | x | sums | the rows' largest numbers | barriers
     const uint32_t x_plane = (uint32_t)most * 4 * p.tokens * 64;
@@ -377,9 +387,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     uint64_t* full = reinterpret_cast<uint64_t*>(largest + 16) + warp * p.depth;
 
     // the warp's records: of its block of rows in every unit, columns w0 ... w1
-    const int wk = warp % p.along_k, wr = warp / p.along_k;
-    const int w0 = c0 + (c1 - c0) * wk / p.along_k, w1 = c0 + (c1 - c0) * (wk + 1) / p.along_k;
-    const int my_rounds = cluster < units ? (units - 1 - cluster) / p.clusters + 1 : 0;
+    const int wk = warp & (along_k - 1), wr = warp >> p.along_shift;
+    const int w0 = c0 + (((c1 - c0) * wk) >> p.along_shift), w1 = c0 + (((c1 - c0) * (wk + 1)) >> p.along_shift);
+    const int my_rounds = cluster < p.units ? (p.units - 1 - cluster) / p.clusters + 1 : 0;
     const int last_unit = cluster + (my_rounds - 1) * p.clusters;
     const int warp_rounds = my_rounds > 0 && last_unit * blocks_per_unit + wr >= p.row_blocks ? my_rounds - 1 : my_rounds;
     int rounds_to_ask = w1 > w0 ? warp_rounds : 0, next_chunk = w0, next_block = cluster * blocks_per_unit + wr;
@@ -412,41 +422,58 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     pdl_wait();
     // (warps / tokens warps to a token)
     const int token_pieces = (c1 - c0) * 16, token_warps = p.warps / tokens;
-    const int token = warp % tokens, first_piece = warp / tokens < token_warps ? (warp / tokens) * 32 + lane : token_pieces;
+    const int token_turn = warp / tokens, token = warp - token_turn * tokens;
+    const int first_piece = token_turn < token_warps ? token_turn * 32 + lane : token_pieces, step = token_warps * 32;
     const T* x_row = static_cast<const T*>(p.x) + (token0 + token) * p.x_stride;
+    uint8_t* x_to = xs + token * 64;
     auto put = [&](int i, const T (&raw)[8], float up_by) {
         float pairs[4][2];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             pairs[j / 2][j % 2] = to_f32(raw[j]) * up_by;
-        uint8_t* dst = xs + ((i >> 2) * p.tokens + token) * 64 + (i & 3) * 16;
+        uint8_t* dst = x_to + (i >> 2) * p.tokens * 64 + (i & 3) * 16;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
             *reinterpret_cast<uint4*>(dst + part * x_plane)
                 = make_uint4(take_half_pair(pairs[0]), take_half_pair(pairs[1]), take_half_pair(pairs[2]), take_half_pair(pairs[3]));
     };
     // once as it is (and rows that want a factor once more)
-    constexpr int AT_ONCE = X32 ? 4 : 8;         // pieces of a thread on their way
     float most_of = 0.f;
-    for (int i0 = first_piece; i0 < token_pieces; i0 += AT_ONCE * token_warps * 32) {
-        T raw[AT_ONCE][8];
+    auto look = [&](const T (&raw)[8]) {
 #pragma unroll
-        for (int a = 0; a < AT_ONCE; ++a) {
-            const int i = i0 + a * token_warps * 32;
-            if (i < token_pieces)
-                read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw[a]);
+        for (int j = 0; j < 8; ++j) {
+            const float v = fabsf(to_f32(raw[j]));
+            most_of = v < INFINITY ? fmaxf(most_of, v) : most_of;
         }
+    };
+    if (((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)p.x_stride * sizeof(T)) & 15) == 0 && (p.k & 7) == 0) {
+        // whole pieces on 16 bytes
+        constexpr int AT_ONCE = X32 ? 2 : 4;     // pieces of a thread on their way
+        const int there = min(token_pieces, (p.k - c0 * PACKED_COLS) >> 3);
+        const T* src = x_row + c0 * PACKED_COLS;
+#pragma unroll 1
+        for (int i0 = first_piece; i0 < token_pieces; i0 += AT_ONCE * step) {
+            __align__(16) T raw[AT_ONCE][8];
 #pragma unroll
-        for (int a = 0; a < AT_ONCE; ++a) {
-            const int i = i0 + a * token_warps * 32;
-            if (i < token_pieces) {
+            for (int a = 0; a < AT_ONCE; ++a)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = fabsf(to_f32(raw[a][j]));
-                    most_of = v < INFINITY ? fmaxf(most_of, v) : most_of;
+                for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+                    reinterpret_cast<uint4*>(raw[a])[h]
+                        = i0 + a * step < there ? reinterpret_cast<const uint4*>(src + (i0 + a * step) * 8)[h] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int a = 0; a < AT_ONCE; ++a)
+                if (i0 + a * step < token_pieces) {
+                    look(raw[a]);
+                    put(i0 + a * step, raw[a], 1.f);
                 }
-                put(i, raw[a], 1.f);
-            }
+        }
+    } else {
+#pragma unroll 1
+        for (int i = first_piece; i < token_pieces; i += step) {
+            T raw[8];
+            read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
+            look(raw);
+            put(i, raw, 1.f);
         }
     }
     const uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
@@ -454,7 +481,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
         atomicMax(&largest[token], warps_most);
     __syncthreads();
     if (const int e = row_exponent(largest[token])) {
-        for (int i = first_piece; i < token_pieces; i += token_warps * 32) {
+#pragma unroll 1
+        for (int i = first_piece; i < token_pieces; i += step) {
             T raw[8];
             read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
             put(i, raw, power_of_two(e));
@@ -571,36 +599,35 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
 
         // ---- the cluster adds up what its warps have
         __syncwarp();
-        if (p.splits > 1)
+        if (splits > 1)
             cluster_sync();
         else
             __syncthreads();
         const int rows_out = p.pair ? PACKED_ROWS / 2 : PACKED_ROWS;
         const int outputs = now * blocks_per_unit * rows_out * tokens;
-        for (int e = rank * blockDim.x + threadIdx.x; e < outputs; e += p.splits * blockDim.x) {
-            const int row = e % rows_out;
-            const int token = e / rows_out % tokens;
-            const int block = e / (rows_out * tokens);                   // of the batch: unit by unit
-            const int u = block / blocks_per_unit, b = block % blocks_per_unit;
+        for (int e = rank * blockDim.x + threadIdx.x; e < outputs; e += splits * blockDim.x) {
+            const int row = e & (rows_out - 1), rest = e >> (p.pair ? 4 : 5);
+            const int block = rest / tokens, token = rest - block * tokens;          // block: of the batch, unit by unit
+            const int u = block >> unit_shift, b = block & (blocks_per_unit - 1);
             const int at = ((cluster + (first + u) * p.clusters) * blocks_per_unit + b) * rows_out + row;
             if (at >= p.n)
                 continue;
             // the fragment's place of (row of the record, token); a pair's up lies two registers behind its gate
             const int in_record = p.pair ? (row >> 3) * 16 + (row & 7) : row;
             const int reg = ((in_record >> 4) * NT + (token >> 3)) * 4 + ((in_record >> 3) & 1) * 2 + (token & 1);
-            const float* place = sums + (u * p.warps + b * p.along_k) * SUMS + reg * 32 + (in_record & 7) * 4 + (token & 7) / 2;
+            const float* place = sums + (u * p.warps + b * along_k) * SUMS + reg * 32 + (in_record & 7) * 4 + (token & 7) / 2;
             float v = 0.f, up = 0.f;
-            if (p.splits > 1) {
+            if (splits > 1) {
                 const uint32_t from = smem_addr(place);
-                for (int s = 0; s < p.splits; ++s)
-                    for (int w = 0; w < p.along_k; ++w) {
+                for (int s = 0; s < splits; ++s)
+                    for (int w = 0; w < along_k; ++w) {
                         v += peer_shared_f32(from + w * (SUMS * 4), s);
                         if (p.pair)
                             up += peer_shared_f32(from + w * (SUMS * 4) + 256, s);
                     }
             } else {
 #pragma unroll 4
-                for (int w = 0; w < p.along_k; ++w) {
+                for (int w = 0; w < along_k; ++w) {
                     v += place[w * SUMS];
                     if (p.pair)
                         up += place[w * SUMS + 64];
@@ -617,7 +644,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
                 static_cast<__nv_bfloat16*>(p.out)[m * p.out_stride + at] = from_f32<__nv_bfloat16>(v);
         }
         __syncwarp();
-        if (p.splits > 1)
+        if (splits > 1)
             cluster_sync();                      // nobody leaves, or writes new sums, while another reads
         else if (first + p.batch < my_rounds)
             __syncthreads();
@@ -631,7 +658,7 @@ void (*few_rows_kernel_of(int group))(const CUtensorMap, const FewRows)
                        : (group == 64 ? packed_few_rows_kernel<NT, X32, 2> : packed_few_rows_kernel<NT, X32, 4>);
 }
 
-constexpr size_t FEW_SMEM_LIMIT = 227 * 1024;
+constexpr size_t FEW_SMEM_LIMIT = 226 * 1024;        // (a timeline build has a word of its own)
 
 size_t few_rows_smem(bool x32, int group, int chunks, int warps, int splits, int batch, int depth, int run, int tokens)
 {
@@ -720,7 +747,7 @@ CHIBI_API int chibi_packed_few_rows_kb(int x32, int group, int cols, int tokens,
 // How many clusters of `splits` CTAs with that much shared memory run at once (0: none, or an error).
 CHIBI_API int chibi_packed_few_rows_clusters(int x32, int group, int tokens, int warps, int splits, int kb)
 {
-    if (!packed_group_ok(group) || splits < 1 || splits > 8 || tokens < 1 || tokens > 16 || kb < 1 || kb > 227 || warps < 1 || warps > 16)
+    if (!packed_group_ok(group) || splits < 1 || splits > 8 || tokens < 1 || tokens > 16 || kb < 1 || kb > 226 || warps < 1 || warps > 16)
         return 0;
     void (*kernel)(const CUtensorMap, const FewRows) = few_rows_kernel(x32 != 0, tokens, group);
     cudaLaunchConfig_t cfg = {};
@@ -768,7 +795,7 @@ CHIBI_API int chibi_packed_few_rows(const ChibiPackedCall* c, const void* x, lon
     const int chunks = (c->k + PACKED_COLS - 1) / PACKED_COLS;
     if ((c->warps != 8 && c->warps != 16) || c->splits < 1 || c->splits > 8 || (c->splits & (c->splits - 1)) || c->splits > chunks
         || c->along_k < 1 || c->along_k > c->warps || (c->along_k & (c->along_k - 1)) || c->batch < 1 || c->depth < 1 || c->run < 1
-        || c->run > 256 || c->tokens < 1 || c->tokens > c->warps || c->clusters < 1)
+        || c->run > 256 || chunks > (1 << 27) || c->tokens < 1 || c->tokens > c->warps || c->clusters < 1)
         return CHIBI_ERR_ARGUMENT;
     const bool x32 = c->x_type == CHIBI_F32;
     const size_t smem = few_rows_smem(x32, c->group, chunks, c->warps, c->splits, c->batch, c->depth, c->run, c->tokens);
@@ -778,9 +805,15 @@ CHIBI_API int chibi_packed_few_rows(const ChibiPackedCall* c, const void* x, lon
         return CHIBI_ERR_UNSUPPORTED;
     CUtensorMap map;
     memcpy(&map, c->map, sizeof(map));
+    int split_shift = 0, along_shift = 0;
+    while ((1 << split_shift) < c->splits)
+        ++split_shift;
+    while ((1 << along_shift) < c->along_k)
+        ++along_shift;
+    const int per_unit = c->warps >> along_shift;
     const FewRows p { row_blocks, chunks, c->n, c->k, c->pair, x, x_stride, c->m, out, c->out_type, out_stride, (const float*)residual,
-                      residual_stride, c->act, c->warps, c->splits, c->along_k, c->batch, c->depth, c->run, c->tokens, c->clusters,
-                      (int*)c->error };
+                      residual_stride, c->act, c->warps, split_shift, along_shift, c->batch, c->depth, c->run, c->tokens, c->clusters,
+                      (row_blocks + per_unit - 1) / per_unit, (int*)c->error };
     void (*kernel)(const CUtensorMap, const FewRows) = few_rows_kernel(x32, c->tokens, c->group);
     static std::atomic<unsigned long long> allowed[2][2][3];
     const cudaError_t e = packed_allow_shared(kernel, allowed[x32][c->tokens <= 8][c->group / 64], FEW_SMEM_LIMIT);
