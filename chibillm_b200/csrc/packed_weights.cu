@@ -460,12 +460,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
                 for (int h = 0; h < (int)sizeof(T) / 2; ++h)
                     reinterpret_cast<uint4*>(raw[a])[h]
                         = i0 + a * step < there ? reinterpret_cast<const uint4*>(src + (i0 + a * step) * 8)[h] : make_uint4(0, 0, 0, 0);
+            // (one copy of the code for all of them: what a kernel runs once it waits for)
+#pragma unroll 1
+            for (int i = i0; i < min(i0 + AT_ONCE * step, token_pieces); i += step) {
+                look(raw[0]);
+                put(i, raw[0], 1.f);
 #pragma unroll
-            for (int a = 0; a < AT_ONCE; ++a)
-                if (i0 + a * step < token_pieces) {
-                    look(raw[a]);
-                    put(i0 + a * step, raw[a], 1.f);
-                }
+                for (int a = 0; a + 1 < AT_ONCE; ++a)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        raw[a][j] = raw[a + 1][j];
+            }
         }
     } else {
 #pragma unroll 1
