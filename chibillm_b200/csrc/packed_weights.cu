@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // How the work is shared out (CudaKernels.packed_plan chooses): `splits` CTAs of a cluster share the columns, `along_k`
 // warps of a CTA share the CTA's columns of one block of 32 rows, the CTA's warps / along_k blocks of rows are a unit, and clusters
 // take units in turn.  The sums of up to `batch` units stay in shared memory; then the cluster adds them up in one order
-// (CTA by CTA, warp by warp), each CTA a share of the outputs, so the same plan gives the same bits.
+// (each CTA its warps, then CTA by CTA), each CTA a share of the outputs, so the same plan gives the same bits.
 constexpr int FEW_THREADS = 512;             // at most
 
 struct FewRows {
@@ -603,11 +603,20 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
         }
 
         // ---- the cluster adds up what its warps have
-        __syncwarp();
-        if (splits > 1)
+        __syncthreads();
+        if (splits > 1) {
+            // a CTA's warps first, in place: another CTA's shared memory is far
+            for (int i = threadIdx.x; i < now * blocks_per_unit * SUMS && along_k > 1; i += blockDim.x) {
+                float* to = sums + (i / SUMS) * along_k * SUMS + i % SUMS;
+                float v = to[0];
+#pragma unroll 4
+                for (int w = 1; w < along_k; ++w)
+                    v += to[w * SUMS];
+                to[0] = v;
+            }
+            __syncwarp();
             cluster_sync();
-        else
-            __syncthreads();
+        }
         const int rows_out = p.pair ? PACKED_ROWS / 2 : PACKED_ROWS;
         const int outputs = now * blocks_per_unit * rows_out * tokens;
         for (int e = rank * blockDim.x + threadIdx.x; e < outputs; e += splits * blockDim.x) {
@@ -624,12 +633,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
             float v = 0.f, up = 0.f;
             if (splits > 1) {
                 const uint32_t from = smem_addr(place);
-                for (int s = 0; s < splits; ++s)
-                    for (int w = 0; w < along_k; ++w) {
-                        v += peer_shared_f32(from + w * (SUMS * 4), s);
-                        if (p.pair)
-                            up += peer_shared_f32(from + w * (SUMS * 4) + 256, s);
-                    }
+                for (int s = 0; s < splits; ++s) {
+                    v += peer_shared_f32(from, s);
+                    if (p.pair)
+                        up += peer_shared_f32(from + 256, s);
+                }
             } else {
 #pragma unroll 4
                 for (int w = 0; w < along_k; ++w) {

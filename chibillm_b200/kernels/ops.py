@@ -189,7 +189,7 @@ class CudaKernels:
         self._attention_tied_libs = {}
         self.use_tcgen05_attention = True
         # matrices in 4 bits: up to so many bfloat16 rows of x stream the matrix once through mma.sync, more go to tcgen05
-        self.packed_few_rows_max = 12
+        self.packed_few_rows_max = 16
         # (by sizes, for all kernels of a process on this device)
         self._packed_plans: Dict[tuple, FewRowsPlan] = _PACKED_PLANS.setdefault(self._device_index, {})
         self._packed_cuts: Dict[tuple, ManyRowsCut] = _PACKED_CUTS.setdefault(self._device_index, {})

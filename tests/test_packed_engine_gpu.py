@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import fokurax_models
+import gitipel_models
 import helpers
 import lefavik_models
 import plain_qwen3
@@ -102,6 +103,26 @@ def test_other_architectures(config):
         requests = helpers.random_requests(spec.vocab_size, [33, 7, 50], seed=9)
         logits.append(helpers.run_trace(runner, helpers.trace_last_decoded(requests, 6)))
     helpers.assert_logits_close(logits[0], logits[1], helpers.TOL["float32"], "4 bits, another architecture")
+
+
+@pytest.mark.parametrize("name", ["G1", "G3"])
+def test_a_recurrent_architecture_cut_in_different_ways(tmp_path, name):
+    """Gitipel: attention and feed-forwards in 4 bits beside a recurrence as it is; whole prompts against single tokens."""
+    config = gitipel_models.get(name)
+    folder = gitipel_models.write_model(config, str(tmp_path / "model"), 4)
+    vocab = int(config["vocab"]) if "vocab" in config else int(config["vocab_size"])
+    requests = helpers.random_requests(vocab, [33, 7, 50], seed=9)
+    logits = []
+    for group in (32, None):
+        runner = runner_of(folder, "float32", group)
+        whole = helpers.run_trace(runner, helpers.trace_whole(requests))
+        helpers.assert_logits_close(helpers.run_trace(runner, helpers.trace_last_decoded(requests, 6)), whole, helpers.TOL["float32"],
+                                    f"4 bits {name} decoded")
+        logits.append(whole)
+    # the matrices did change, and not by much
+    for rid in requests:
+        off = float((logits[0][rid] - logits[1][rid]).norm() / logits[1][rid].norm())
+        assert 1e-3 < off < 0.7, off
 
 
 def parts_of(model):
