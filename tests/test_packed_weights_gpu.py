@@ -376,3 +376,173 @@ def test_refusals(kernels):
         with pytest.raises(KernelError):
             call()
     assert kernels.linear_partial(x, packed) is None
+
+
+def test_the_first_call_may_be_captured(kernels):
+    """Nothing that a product asks of the device on its first call stands in a capture's way."""
+    g = gen(30)
+    w = matrix(g, 333, 640, BF16)
+    values = packed_values(w, 64)
+    stream = torch.cuda.Stream()
+    for m, dtype in ((3, BF16), (90, BF16), (5, F32)):
+        packed = kernels.pack_weights(w, 64)
+        x = torch.randn(m, 640, generator=g, device=DEV).to(dtype)
+        out = torch.empty(m, 333, device=DEV)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            kernels.linear(x, packed, out)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = x.double() @ values.t()
+        close(out, want, off_by(x, values, 64, F32, want))
+
+
+def test_packing_inside_a_capture_and_its_product_at_once(kernels):
+    g = gen(31)
+    w = matrix(g, 256, 512, BF16)
+    x = torch.randn(4, 512, generator=g, device=DEV).to(BF16)
+    out = torch.empty(4, 256, device=DEV)
+    kernels.linear(x, kernels.pack_weights(w, 32), out)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        packed = kernels.pack_weights(w, 32)
+        kernels.linear(x, packed, out)
+    for _ in range(20):
+        w.copy_(matrix(g, 256, 512, BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        values = packed_values(w, 32)
+        want = x.double() @ values.t()
+        close(out, want, off_by(x, values, 32, F32, want))
+
+
+@pytest.mark.parametrize("m", [1, 9, 60])
+def test_the_first_rows_of_a_matrix(kernels, m):
+    g = gen(32)
+    w = matrix(g, 300, 256, BF16)
+    packed = kernels.pack_weights(w, 64)
+    x = torch.randn(m, 256, generator=g, device=DEV).to(BF16)
+    whole = torch.empty(m, 300, device=DEV)
+    kernels.linear(x, packed, whole)
+    for n in (1, 32, 45, 299, 300):
+        out = torch.full((m, n + 3), 5.0, device=DEV)
+        kernels.linear(x, packed[:n], out[:, :n])
+        values = packed_values(w, 64)[:n]
+        want = x.double() @ values.t()
+        close(out[:, :n], want, off_by(x, values, 64, F32, want))
+        assert (out[:, n:] == 5).all()
+
+
+def test_rows_whose_factor_is_still_to_be_applied(kernels):
+    """A norm's output without its rows' factor, as the bfloat16 products of many rows leave it."""
+    g = gen(33)
+    a, w0 = torch.randn(300, 256, generator=g, device=DEV).to(BF16), matrix(g, 512, 256, BF16)
+    residual = torch.randn(300, 512, generator=g, device=DEV)
+    norm = torch.ones(512, device=DEV)
+    scaled = kernels.linear_residual_norm(a, w0, residual, norm, 1e-6, 0.0, torch.empty(300, 512, dtype=BF16, device=DEV))
+    assert scaled is not None
+    w = matrix(g, 200, 512, BF16)
+    packed, values = kernels.pack_weights(w, 64), packed_values(w, 64)
+    out = torch.empty(300, 200, device=DEV)
+    kernels.linear(scaled, packed, out)
+    x = scaled.materialise()
+    want = x.double() @ values.t()
+    close(out, want, off_by(x, values, 64, F32, want))
+
+
+@pytest.mark.parametrize("m", [4, 40])
+def test_bfloat16_rows_of_every_size(kernels, m):
+    g = gen(34)
+    w = matrix(g, 100, 384, BF16)
+    packed, values = kernels.pack_weights(w, 64), packed_values(w, 64)
+    x = torch.randn(m, 384, generator=g, device=DEV)
+    x *= (10.0 ** torch.linspace(-30, 30, m, device=DEV))[:, None]
+    x[0, :200] *= 1e-4
+    x = x.to(BF16)
+    out = torch.empty(m, 100, device=DEV)
+    kernels.linear(x, packed, out)
+    want = x.double() @ values.t()
+    # (few rows: numbers below 2^-29 of a row's largest are off by 2^-40 of it, 2^-25 where that is 1 ... 2^15)
+    small = x.double().abs().amax(1, keepdim=True) * 2.0 ** -25 * values.abs().sum(1)[None, :]
+    close(out, want, off_by(x, values, 64, F32, want) + small)
+
+
+def test_infinities_in_many_rows(kernels):
+    g = gen(35)
+    w = matrix(g, 130, 256, BF16)
+    packed, values = kernels.pack_weights(w, 32), packed_values(w, 32)
+    x = torch.randn(50, 256, generator=g, device=DEV).to(BF16)
+    clean, out = torch.empty(50, 130, device=DEV), torch.empty(50, 130, device=DEV)
+    kernels.linear(x, packed, clean)
+    x[11, 17], x[30, 200], x[49, 3] = math.inf, math.nan, -math.inf
+    kernels.linear(x, packed, out)
+    rest = [i for i in range(50) if i not in (11, 30, 49)]
+    assert torch.equal(out[rest], clean[rest]) and out[30].isnan().all()
+    for row, at, sign in ((11, 17, 1.0), (49, 3, -1.0)):
+        v = values[:, at]
+        assert out[row][v == 0].isnan().all()
+        assert torch.equal(out[row][v != 0], (sign * v[v != 0].sign() * math.inf).float())
+
+
+def test_outputs_and_matrices_beyond_32_bits(kernels):
+    """More than 2^31 outputs, and a matrix of more than 2^31 elements."""
+    g = gen(36)
+    w = matrix(g, 151936, 64, BF16)
+    packed = kernels.pack_weights(w, 64)
+    m = 14200
+    x = torch.randn(m, 64, generator=g, device=DEV).to(BF16)
+    out = torch.empty(m, 151936, dtype=BF16, device=DEV)
+    kernels.linear(x, packed, out)
+    rows = [0, 1, m // 2, m - 2, m - 1]
+    few = torch.empty(len(rows), 151936, dtype=BF16, device=DEV)
+    kernels.linear(x[rows].contiguous(), packed, few)
+    # (other orders of the sums: a rounding apart at most)
+    assert ((out[rows].float() - few.float()).abs() <= few.float().abs() * 2.0 ** -7 + 1e-6).all()
+    del out
+    n, k = 70016, 32768
+    w = torch.empty(n, k, dtype=BF16, device=DEV).normal_(0.0, 0.02, generator=g)
+    packed = kernels.pack_weights(w, 128)
+    x = torch.randn(2, k, generator=g, device=DEV).to(BF16)
+    out = torch.empty(2, n, device=DEV)
+    kernels.linear(x, packed, out)
+    for at in (0, 35000, n - 40):
+        part = w[at:at + 40].contiguous()
+        values = packed_values(part, 128)
+        want = x.double() @ values.t()
+        close(out[:, at:at + 40], want, off_by(x, values, 128, F32, want))
+    kernels.check_error_word()
+
+
+def test_calls_from_two_threads(kernels):
+    import threading
+    g = gen(37)
+    w = matrix(g, 1000, 1024, BF16)
+    packed = kernels.pack_weights(w, 64)
+    x = {m: torch.randn(m, 1024, generator=g, device=DEV).to(BF16) for m in range(1, 60)}
+    want = {}
+    for m in x:
+        want[m] = torch.empty(m, 1000, device=DEV)
+        kernels.linear(x[m], packed, want[m])
+    torch.cuda.synchronize()
+    packed.calls.clear()
+    wrong = []
+
+    def work(order):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            outs = []
+            for m in order:
+                out = torch.empty(m, 1000, device=DEV)
+                kernels.linear(x[m], packed, out)
+                outs.append((m, out))
+        stream.synchronize()
+        wrong.extend(m for m, out in outs if not torch.equal(out, want[m]))
+
+    threads = [threading.Thread(target=work, args=(list(x)[::step],)) for step in (1, -1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
