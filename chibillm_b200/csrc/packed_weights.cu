@@ -286,11 +286,11 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // multiplied by the scales in 32 bits.
 //
 // x becomes float16 too (two nibbles of a word are float16 numbers without a shift, which bfloat16's seven bits of mantissa
-// do not allow; the conversion of the codes is most of the kernel's instructions).  A row whose largest number of the CTA's
-// columns is not within 1 ... 2^15 is multiplied by the power of two that brings it to 2^14 ... 2^15, and its sums by the inverse: so
-// bfloat16 numbers from 2^-14 (of a scaled row: 2^-29 of the largest) on keep all of their bits, smaller ones are off by 2^-25 (2^-40) at
-// most.  32-bit numbers are two float16 numbers, the nearest and the nearest to what is left: off by 2^-23 of themselves or
-// by 2^-25 of the row's largest at most, no more than the 32-bit sums lose.
+// do not allow; the conversion of the codes is most of the kernel's instructions).  A row of bfloat16 whose largest number of the CTA's
+// columns is not within 1 ... 2^15, and every row of 32-bit numbers, is multiplied by the power of two that brings the largest to
+// 2^14 ... 2^15, and its sums by the inverse.  So bfloat16 numbers from 2^-14 (of a scaled row: 2^-29 of the largest) on keep all of their
+// bits, smaller ones are off by 2^-25 (2^-40) at most.  32-bit numbers are two float16 numbers, the nearest and the nearest to what is
+// left: off by 2^-23 of themselves or by 2^-40 of the row's largest at most, no more than the 32-bit sums lose.
 //
 // How the work is shared out (CudaKernels.packed_plan chooses): `splits` CTAs of a cluster share the columns, `along_k`
 // warps of a CTA share the CTA's columns of one block of 32 rows, the CTA's warps / along_k blocks of rows are a unit, and clusters
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 //
 // Measured (replayed in a graph, matrices out of L2): one row of 2,048 x 1,024 3.0 us, of 4,096 x 4,096 4.7, of 4,096 x 12,288 8.9, of a gated
 // pair of 2 x 12,288 x 4,096 13.0 (4.1 TB/s); four rows of 151,936 x 4,096 63.7 (5.2 TB/s), 284 instructions a record at 2.55 a
-// cycle and SM; 12 32-bit rows of a pair of 2 x 2,730 x 1,024 5.8.  Before and after the stream of one row go by 2.5 us: a kernel's start, x from
+// cycle and SM; 12 32-bit rows of a pair of 2 x 2,730 x 1,024 6.4.  Before and after the stream of one row go by 2.5 us: a kernel's start, x from
 // L2, a barrier, the warps' sums.
 constexpr int FEW_THREADS = 512;             // at most
 
@@ -341,12 +341,12 @@ __device__ __forceinline__ float peer_shared_f32(uint32_t own_smem_addr, uint32_
     return v;
 }
 
-// The exponent of the power of two by which a row is multiplied, from its largest finite magnitude: none where that is
-// 1 ... 2^15, else the one that brings it to 2^14 ... 2^15 (as far as a 32-bit number goes: rows below 2^-112 come out smaller).
-__device__ __forceinline__ int row_exponent(uint32_t largest_bits)
+// The exponent of the power of two by which a row is multiplied, from its largest finite magnitude: the one that brings it to
+// 2^14 ... 2^15 (as far as a 32-bit number goes: rows below 2^-112 come out smaller), for bfloat16 none where it is 1 ... 2^15.
+template <bool X32> __device__ __forceinline__ int row_exponent(uint32_t largest_bits)
 {
     const int e = (int)(largest_bits >> 23) - 127;
-    return (e >= 0 && e < 15) || largest_bits == 0 ? 0 : min(14 - e, 126);
+    return (!X32 && e >= 0 && e < 15) || largest_bits == 0 ? 0 : min(14 - e, 126);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
             *reinterpret_cast<uint4*>(dst + part * x_plane)
                 = make_uint4(take_half_pair(pairs[0]), take_half_pair(pairs[1]), take_half_pair(pairs[2]), take_half_pair(pairs[3]));
     };
-    // once as it is (and rows that want a factor once more)
+    // bfloat16 rows once as they are, and those that want a factor once more; 32-bit rows when the factor is known
     float most_of = 0.f;
     auto look = [&](const T (&raw)[8]) {
 #pragma unroll
@@ -469,7 +469,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
 #pragma unroll 1
             for (int i = i0; i < min(i0 + AT_ONCE * step, token_pieces); i += step) {
                 look(raw[0]);
-                put(i, raw[0], 1.f);
+                if constexpr (!X32)
+                    put(i, raw[0], 1.f);
 #pragma unroll
                 for (int a = 0; a + 1 < AT_ONCE; ++a)
 #pragma unroll
@@ -483,14 +484,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
             T raw[8];
             read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
             look(raw);
-            put(i, raw, 1.f);
+            if constexpr (!X32)
+                put(i, raw, 1.f);
         }
     }
     const uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
     if (lane == 0)
         atomicMax(&largest[token], warps_most);
     __syncthreads();
-    if (const int e = row_exponent(largest[token])) {
+    if (const int e = row_exponent<X32>(largest[token]); X32 || e != 0) {
 #pragma unroll 1
         for (int i = first_piece; i < token_pieces; i += step) {
             T raw[8];
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
         x_lane[t] = (uint32_t)min(t * 8 + r, tokens - 1) * 64 + c * 16;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            down[t][j] = power_of_two(-row_exponent(largest[min(t * 8 + 2 * c + j, tokens - 1)]));
+            down[t][j] = power_of_two(-row_exponent<X32>(largest[min(t * 8 + 2 * c + j, tokens - 1)]));
     }
     const uint32_t x_block = (uint32_t)p.tokens * 64;
     bool dead = false;                           // a wait ran out: nothing more is asked for

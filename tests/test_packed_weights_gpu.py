@@ -546,3 +546,25 @@ def test_calls_from_two_threads(kernels):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+@pytest.mark.parametrize("m", [1, 10, 30])
+def test_small_numbers_beside_a_large_one_that_no_weight_sees(kernels, m, x_dtype):
+    """A row's largest number meets zeros; the others are float16 subnormals beside it.  bfloat16 of few rows: off by 2^-25 of the
+    largest (2^-40 where it is beyond 2^15); 32-bit: by 2^-40."""
+    g = gen(40)
+    w = matrix(g, 64, 384, BF16)
+    w[:, 7] = 0.0
+    packed, values = kernels.pack_weights(w, 64), packed_values(w, 64)
+    assert (values[:, 7] == 0).all()
+    for largest in (1.5, 3e4, 1e8):
+        x = (torch.randn(m, 384, generator=g, device=DEV) * (1e-5 * largest)).to(x_dtype)
+        x[:, 7] = largest
+        out = torch.empty(m, 64, device=DEV)
+        kernels.linear(x, packed, out)
+        want = x.double() @ values.t()
+        unseen = x.clone()
+        unseen[:, 7] = 0.0
+        step = largest * 2.0 ** -25 if x_dtype == BF16 and largest < 2.0 ** 15 else largest * 2.0 ** -40
+        close(out, want, off_by(unseen, values, 64, F32, want) + step * values.abs().sum(1)[None, :])
