@@ -72,7 +72,11 @@ def few_rows_plan(rows: int, columns: int, paired: bool, m: int, wide: bool, sme
     to 151,936 x 4,096): a record takes an SM 60 and a warp 530 (what instructions it issues, and their latency), two instructions
     for every 8 rows of x more of it; adding up the sums of a round 400; a cluster that adds up across CTAs 1,200.  About 64
     records are to be on their way to an SM (at 32, 4,096 x 12,288 took 13.3 us instead of 10.2), and no more room is taken than
-    a warp's records need, so that the next kernel's CTAs fit beside (2,051 x 1,021: 6.2 us with four places a warp, 4.4 with one)."""
+    a warp's records need, so that the next kernel's CTAs fit beside (2,051 x 1,021: 6.2 us with four places a warp, 4.4 with one).
+
+    With more rows of x than a CTA holds, their blocks are the grid's second axis, and what does not run at once runs after it:
+    counted as whole waves (32-bit prompts, and bfloat16 ones of odd widths; uncounted, larger clusters looked as cheap as none: 1,024
+    bfloat16 rows of 4,096 x 4,095 401 us instead of 185, 2,000 32-bit rows 1,015 instead of 589)."""
     blocks = -(-rows // (BLOCK_ROWS // 2 if paired else BLOCK_ROWS))
     chunks = -(-columns // BLOCK_COLS)
     tokens = -(-m // -(-m // FEW_TOKENS))
@@ -102,12 +106,14 @@ def few_rows_plan(rows: int, columns: int, paired: bool, m: int, wide: bool, sme
                     kb = smem_kb(tokens, warps, splits, 1, depth, run)
                     if kb > room:
                         continue
-                    clusters = min(units, max(1, most_clusters(tokens, warps, splits, kb) // token_blocks))
+                    at_once = max(1, most_clusters(tokens, warps, splits, kb))
+                    clusters = min(units, max(1, at_once // token_blocks))
                     rounds = -(-units // clusters)
+                    waves = -(-clusters * token_blocks // at_once)
                     on_sm = -(-clusters * splits // sms)
                     busy = on_sm * per_unit * min(along_k, mine)
-                    time = on_sm * rounds * per_unit * mine * max(issue, 530 / busy) + rounds * 400 + (1200 if splits > 1 else 0) \
-                        + mine * 16 * tokens / (warps * 32) * 30
+                    time = waves * (on_sm * rounds * per_unit * mine * max(issue, 530 / busy) + rounds * 400
+                                    + (1200 if splits > 1 else 0) + mine * 16 * tokens / (warps * 32) * 30)
                     if best is None or time < best[0]:
                         best = (time, FewRowsPlan(warps, splits, along_k, 1, depth, run, tokens, clusters), rounds, room)
         if best is not None:

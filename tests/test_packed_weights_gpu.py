@@ -568,3 +568,11 @@ def test_small_numbers_beside_a_large_one_that_no_weight_sees(kernels, m, x_dtyp
         unseen[:, 7] = 0.0
         step = largest * 2.0 ** -25 if x_dtype == BF16 and largest < 2.0 ** 15 else largest * 2.0 ** -40
         close(out, want, off_by(unseen, values, 64, F32, want) + step * values.abs().sum(1)[None, :])
+
+
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(700, 65, 515), (2400, 100, 129), (5000, 33, 1001)])
+def test_more_blocks_of_rows_than_run_at_once(kernels, m, n, k, x_dtype):
+    """Odd widths and 32-bit rows: 16 rows of x a CTA, more CTAs than there are SMs."""
+    check_product(kernels, m, n, k, 64, x_dtype, F32, residual=True)
+    check_gated(kernels, m, n, k, 64, x_dtype, "silu")
