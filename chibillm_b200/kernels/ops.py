@@ -810,6 +810,7 @@ class CudaKernels:
 
     def _pack(self, w: torch.Tensor, up: Optional[torch.Tensor], group: int, what: str) -> PackedWeights:
         self._packed_sizes(w, group, what)
+        self._on_this_device(what, up)
         for t in (w, up):
             if t is not None:
                 _rows_contiguous(t, what)

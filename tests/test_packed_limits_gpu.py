@@ -1,0 +1,27 @@
+"""Matrices in 4 bits on the device: the calls at the edge of what the operators take.
+
+Comparisons are with the definition in 64 bits.  What a product of few rows may be off by is ``off_by`` of
+test_packed_weights_gpu.py; where whole numbers make every sum exact, bits have to be equal.
+"""
+import math
+
+import pytest
+import torch
+
+from test_packed_weights_gpu import BF16, DEV, F32, close, gen, matrix, off_by, packed_values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kernels():
+    from chibillm_b200.kernels.ops import CudaKernels
+    return CudaKernels(torch.device(DEV))
+
+
+def test_a_pair_whose_second_matrix_is_elsewhere_is_refused(kernels):
+    from chibillm_b200.kernels.ops import KernelError
+    w = torch.zeros(32, 64, dtype=BF16, device=DEV)
+    for gate, up in ((w, w.cpu()), (w.cpu(), w)):
+        with pytest.raises(KernelError):
+            kernels.pack_gate_up(gate, up, 32)
