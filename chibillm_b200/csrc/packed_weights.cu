@@ -85,8 +85,9 @@ template <typename T> __device__ __forceinline__ void read_eight(const T* row, i
     }
 }
 
-// Products fetch their matrix before the kernel ahead of them has ended.  So the kernels that write one let nothing start early
-// (no pdl_trigger; and no mark in a timeline), and every thread's stores are performed, for tile copies too, before it ends.
+// Products fetch their matrix before the kernel ahead of them has ended.  So the kernels that write one, in 4 bits or as values read
+// back, let nothing start early (no pdl_trigger; and no mark in a timeline), and every thread's stores are performed, for tile copies
+// too, before it ends.
 __device__ __forceinline__ void packed_done()
 {
     __threadfence();
@@ -226,7 +227,7 @@ template <typename T>
 __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restrict__ data, int row_blocks, int col_blocks, int group, int rows,
                                                      int cols, int pair, T* __restrict__ out, long long stride)
 {
-    pdl_enter();
+    pdl_wait_now();                                  // (see packed_done)
     constexpr int EACH = 16 / sizeof(T), ROW_THREADS = PACKED_COLS / EACH, TURNS = PACKED_ROWS * ROW_THREADS / 512;
     uint32_t next_word[TURNS];
     __nv_bfloat16 next_scale[TURNS];
@@ -274,6 +275,7 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
                     dst[j] = v[j];
         }
     }
+    packed_done();
 }
 
 // ------------------------------------------------------------------ few rows of x

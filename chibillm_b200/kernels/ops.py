@@ -851,7 +851,8 @@ class CudaKernels:
         return out
 
     def unpack_weights(self, w: PackedWeights, out: torch.Tensor) -> None:
-        """The values of a matrix in 4 bits, rounded to out's type; of a pair, gate's rows before up's."""
+        """The values of a matrix in 4 bits, rounded to out's type; of a pair, gate's rows before up's.  ``out`` may be the matrix
+        of the very next product on the stream."""
         self._on_this_device("unpack_weights", w.data, out)
         _rows_contiguous(out, "unpack_weights: out")
         if out.shape != w.shape:

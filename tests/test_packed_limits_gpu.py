@@ -25,3 +25,23 @@ def test_a_pair_whose_second_matrix_is_elsewhere_is_refused(kernels):
     for gate, up in ((w, w.cpu()), (w.cpu(), w)):
         with pytest.raises(KernelError):
             kernels.pack_gate_up(gate, up, 32)
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_values_read_back_are_the_next_products_matrix(kernels, m):
+    """bfloat16 products fetch their matrix early: not before it has been written."""
+    g = gen(50)
+    x = torch.randn(m, 512, generator=g, device=DEV).to(BF16)
+    matrices = [kernels.pack_weights(matrix(g, 2048, 512, BF16), 64) for _ in range(4)]
+    values, out = torch.empty(2048, 512, dtype=BF16, device=DEV), torch.empty(m, 2048, device=DEV)
+    want = []
+    for packed in matrices:
+        kernels.unpack_weights(packed, values)
+        torch.cuda.synchronize()
+        kernels.linear(x, values, out)
+        want.append(out.clone())
+    for turn in range(40):
+        kernels.unpack_weights(matrices[turn % 4], values)
+        kernels.linear(x, values, out)
+        got = out.clone()
+        assert torch.equal(got, want[turn % 4]), turn
