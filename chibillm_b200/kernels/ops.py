@@ -854,6 +854,7 @@ class CudaKernels:
         """The values of a matrix in 4 bits, rounded to out's type; of a pair, gate's rows before up's.  ``out`` may be the matrix
         of the very next product on the stream."""
         self._on_this_device("unpack_weights", w.data, out)
+        self._packed_bytes(w, "unpack_weights")
         _rows_contiguous(out, "unpack_weights: out")
         if out.shape != w.shape:
             raise KernelError(f"unpack_weights: out {tuple(out.shape)}, the matrix is {tuple(w.shape)}")
@@ -886,6 +887,13 @@ class CudaKernels:
     def _packed_room(self, rows: int, columns: int, group: int, paired: bool) -> PackedWeights:
         data = torch.empty(PackedWeights.bytes_for(rows, columns, group, paired), dtype=torch.uint8, device=self.device)
         return PackedWeights(data, rows, columns, group, paired)
+
+    @staticmethod
+    def _packed_bytes(w: PackedWeights, what: str) -> None:
+        need = PackedWeights.bytes_for(w.rows, w.columns, w.group, w.paired)
+        if w.data.dtype != torch.uint8 or not w.data.is_contiguous() or w.data.numel() < need or w.data.data_ptr() % 16:
+            raise KernelError(f"{what}: the matrix's records are {need} neighbouring bytes that start on 16, "
+                              f"got {w.data.numel()} of {w.data.dtype} at {w.data.data_ptr():#x}")
 
     def packed_plan(self, w: PackedWeights, m: int, x32: bool) -> FewRowsPlan:
         """How the product of m rows of x with this matrix is shared out (kernels/packed.py)."""
@@ -935,6 +943,7 @@ class CudaKernels:
         _rows_contiguous(x, f"{what}: x")
         if x.shape[1] != w.columns:
             raise KernelError(f"{what}: shapes x {tuple(x.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
+        self._packed_bytes(w, what)
         m, x_code = x.shape[0], _code(x)
         call = library.PackedCall(_ptr(w.data), _ptr(self.error), w.group, w.rows, w.columns, int(w.paired), m, x_code, _code(out),
                                   self.ACTIVATIONS[kind] if kind else 0)

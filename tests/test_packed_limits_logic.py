@@ -7,6 +7,7 @@ import torch
 
 import chibillm_b200.csrc
 from chibillm_b200.kernels.ops import CudaKernels, KernelError
+from chibillm_b200.kernels.packed import PackedWeights
 
 
 def bare_kernels():
@@ -47,3 +48,24 @@ def test_kernels_that_write_a_matrix_let_no_product_start_early():
     for name in writers:
         assert "pdl_enter()" not in bodies[name] and "pdl_trigger" not in bodies[name], name
         assert bodies[name].lstrip().startswith("pdl_wait_now();") and "packed_done();" in bodies[name], name
+
+
+@pytest.mark.parametrize("paired", [False, True])
+def test_records_that_are_not_all_there_are_refused(monkeypatch, paired):
+    """A kernel reads as many bytes as the matrix's sizes say."""
+    k = bare_kernels()
+    monkeypatch.setattr(k, "_on_this_device", lambda what, *tensors: None)
+    k._current_device = lambda: (_ for _ in ()).throw(AssertionError("a launch"))
+    k.error, k.lib, k.packed_few_rows_max = torch.zeros(1, dtype=torch.int32), None, 16
+    rows, columns, group = 40, 200, 64
+    need = PackedWeights.bytes_for(rows, columns, group, paired)
+    whole = torch.zeros(need + 16, dtype=torch.uint8)
+    whole = whole[-whole.data_ptr() % 16:][:need]
+    x, out = torch.zeros(3, columns), torch.zeros(2 * rows if paired else rows, columns)
+    for data in (whole[:-1], whole[:0], whole[1:], torch.zeros(need, dtype=torch.int8), torch.zeros(2 * need, dtype=torch.uint8)[::2],
+                 torch.cat([whole, whole])[1:]):
+        w = PackedWeights(data, rows, columns, group, paired)
+        with pytest.raises(KernelError, match="bytes"):
+            k.unpack_weights(w, out)
+        with pytest.raises(KernelError, match="bytes"):
+            k._packed_call(x, w, torch.zeros(3, rows), "silu" if paired else None, False, "linear")
