@@ -47,7 +47,7 @@ def make_runtime(dtype, device="cuda:0", kernels=None, spec=None, weight_group: 
     may pass a stand-in for the kernels (then any device is allowed).  With the
     model's ``spec`` the libraries it will load are built together first."""
     device = torch.device(device)
-    if weight_group is not None and weight_group not in WEIGHT_GROUPS:
+    if weight_group is not None and (not isinstance(weight_group, int) or weight_group not in WEIGHT_GROUPS):
         raise ValueError(f"weight_group {weight_group}: matrices in 4 bits have groups of one of {WEIGHT_GROUPS} columns")
     if kernels is None:
         from ..kernels.ops import CudaKernels

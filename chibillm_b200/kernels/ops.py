@@ -878,7 +878,7 @@ class CudaKernels:
                 raise KernelError(f"{what}: a tensor on {t.device}, these kernels run on cuda:{self._device_index}")
 
     def _packed_sizes(self, w: torch.Tensor, group: int, what: str) -> None:
-        if group not in GROUPS:
+        if not isinstance(group, int) or group not in GROUPS:
             raise KernelError(f"{what}: groups of {group} columns (one of {GROUPS})")
         if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
             raise KernelError(f"{what}: a matrix of {tuple(w.shape)}")

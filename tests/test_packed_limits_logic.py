@@ -6,8 +6,10 @@ import pytest
 import torch
 
 import chibillm_b200.csrc
+from chibillm_b200.engine.runner import make_runtime
 from chibillm_b200.kernels.ops import CudaKernels, KernelError
 from chibillm_b200.kernels.packed import PackedWeights
+from packed_models import PackedReferenceKernels
 
 
 def bare_kernels():
@@ -69,3 +71,17 @@ def test_records_that_are_not_all_there_are_refused(monkeypatch, paired):
             k.unpack_weights(w, out)
         with pytest.raises(KernelError, match="bytes"):
             k._packed_call(x, w, torch.zeros(3, rows), "silu" if paired else None, False, "linear")
+
+
+@pytest.mark.parametrize("group", [64.0, True, "64", None, 0, 48, 256])
+def test_groups_are_whole_numbers_of_the_list(monkeypatch, group):
+    k = bare_kernels()
+    monkeypatch.setattr(k, "_on_this_device", lambda what, *tensors: None)
+    w = torch.zeros(32, 64)
+    for call in (lambda: k.pack_weights(w, group), lambda: k.pack_gate_up(w, w, group),
+                 lambda: k.pack_codes(w.to(torch.int8), torch.zeros(32, 1, dtype=torch.bfloat16), group)):
+        with pytest.raises(KernelError, match="groups of"):
+            call()
+    if group is not None:
+        with pytest.raises(ValueError, match="weight_group"):
+            make_runtime("bfloat16", "cpu", kernels=PackedReferenceKernels(), weight_group=group)
