@@ -895,6 +895,14 @@ class CudaKernels:
             raise KernelError(f"{what}: the matrix's records are {need} neighbouring bytes that start on 16, "
                               f"got {w.data.numel()} of {w.data.dtype} at {w.data.data_ptr():#x}")
 
+    @staticmethod
+    def _packed_clusters(asked: tuple, ask) -> int:
+        # (0 may be an error that passes: it is not kept)
+        clusters = _PACKED_CLUSTERS.get(asked) or ask()
+        if clusters > 0:
+            _PACKED_CLUSTERS[asked] = clusters
+        return clusters
+
     def packed_plan(self, w: PackedWeights, m: int, x32: bool) -> FewRowsPlan:
         """How the product of m rows of x with this matrix is shared out (kernels/packed.py)."""
         key = (w.rows, w.columns, w.paired, w.group, m, x32)
@@ -904,15 +912,13 @@ class CudaKernels:
 
             def most_clusters(tokens, warps, splits, kb):
                 # (an instantiation takes up to 8 tokens, or up to 16)
-                asked = (self._device_index, x, w.group, tokens <= 8, warps, splits, kb)
-                if asked not in _PACKED_CLUSTERS:
-                    _PACKED_CLUSTERS[asked] = lib.chibi_packed_few_rows_clusters(x, w.group, tokens, warps, splits, kb)
-                return _PACKED_CLUSTERS[asked]
+                return self._packed_clusters((self._device_index, x, w.group, tokens <= 8, warps, splits, kb),
+                                             lambda: lib.chibi_packed_few_rows_clusters(x, w.group, tokens, warps, splits, kb))
 
             plan = few_rows_plan(w.rows, w.columns, w.paired, m, x32,
                                  lambda *cut: lib.chibi_packed_few_rows_kb(x, w.group, w.columns, *cut), most_clusters, self.sm_count)
             if plan is None:
-                raise KernelError(f"a product over {w.columns} columns in 4 bits: more than the kernel holds")
+                raise KernelError(f"a product over {w.columns} columns in 4 bits: more than the kernel holds, or than the device runs")
             if len(self._packed_plans) > 4096:
                 self._packed_plans.clear()
             self._packed_plans[key] = plan
@@ -924,12 +930,11 @@ class CudaKernels:
         cut = self._packed_cuts.get(key)
         if cut is None:
             def most_clusters(splits):
-                asked = (self._device_index, splits)
-                if asked not in _PACKED_CLUSTERS:
-                    _PACKED_CLUSTERS[asked] = self.lib.chibi_packed_many_rows_clusters(splits)
-                return _PACKED_CLUSTERS[asked]
+                return self._packed_clusters((self._device_index, splits), lambda: self.lib.chibi_packed_many_rows_clusters(splits))
 
             cut = many_rows_cut(w.rows, w.columns, w.paired, m, most_clusters)
+            if cut is None:
+                raise KernelError("a product of many rows with a matrix in 4 bits: the device runs none of its blocks")
             if len(self._packed_cuts) > 4096:
                 self._packed_cuts.clear()
             self._packed_cuts[key] = cut

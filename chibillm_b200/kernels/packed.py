@@ -66,7 +66,8 @@ class FewRowsPlan(NamedTuple):
 def few_rows_plan(rows: int, columns: int, paired: bool, m: int, wide: bool, smem_kb: Callable[..., int],
                   most_clusters: Callable[[int, int, int, int], int], sms: int) -> Optional[FewRowsPlan]:
     """How CTAs and warps share a product of m rows of x (``wide``: 32-bit ones).  ``smem_kb(tokens, warps, splits, batch, depth,
-    run)`` is a CTA's shared memory, ``most_clusters(tokens, warps, splits, kb)`` how many clusters run at once.  None if nothing fits.
+    run)`` is a CTA's shared memory, ``most_clusters(tokens, warps, splits, kb)`` how many clusters run at once (0: none).  None if
+    nothing fits.
 
     The cut with the least time by a rough model, in ns, fitted to sweeps of all cuts (1 to 16 rows of x, matrices of 2,048 x 1,024
     to 151,936 x 4,096): a record takes an SM 60 and a warp 530 (what instructions it issues, and their latency), two instructions
@@ -106,7 +107,9 @@ def few_rows_plan(rows: int, columns: int, paired: bool, m: int, wide: bool, sme
                     kb = smem_kb(tokens, warps, splits, 1, depth, run)
                     if kb > room:
                         continue
-                    at_once = max(1, most_clusters(tokens, warps, splits, kb))
+                    at_once = most_clusters(tokens, warps, splits, kb)
+                    if at_once < 1:
+                        continue
                     clusters = min(units, max(1, at_once // token_blocks))
                     rounds = -(-units // clusters)
                     waves = -(-clusters * token_blocks // at_once)
@@ -134,10 +137,10 @@ class ManyRowsCut(NamedTuple):
     clusters: int
 
 
-def many_rows_cut(rows: int, columns: int, paired: bool, m: int, most_clusters: Callable[[int], int]) -> ManyRowsCut:
+def many_rows_cut(rows: int, columns: int, paired: bool, m: int, most_clusters: Callable[[int], int]) -> Optional[ManyRowsCut]:
     """How tiles of the product with many rows of x are shared out: whole rounds of tiles on all SMs, what is left by clusters
     whose CTAs share a tile's columns.  ``most_clusters(splits)``: how many clusters of so many CTAs run at once (the larger
-    they are, the fewer SMs they reach)."""
+    they are, the fewer SMs they reach).  None if the device runs none of any size."""
     tokens = 48 if m <= 48 else 96 if m <= 96 else 192
     tiles = -(-rows // (64 if paired else 128)) * -(-m // tokens)
     chunks = -(-columns // BLOCK_COLS)
@@ -159,4 +162,4 @@ def many_rows_cut(rows: int, columns: int, paired: bool, m: int, most_clusters: 
             cost, cut = rounds * chunks + -(-chunks // splits) + 3, ManyRowsCut(tokens, rounds, splits, clusters)
         if best is None or cost < best[0]:
             best = (cost, cut)
-    return best[1]
+    return best[1] if best is not None else None

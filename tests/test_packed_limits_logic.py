@@ -8,8 +8,23 @@ import torch
 import chibillm_b200.csrc
 from chibillm_b200.engine.runner import make_runtime
 from chibillm_b200.kernels.ops import CudaKernels, KernelError
-from chibillm_b200.kernels.packed import PackedWeights
+from chibillm_b200.kernels import ops
+from chibillm_b200.kernels.packed import PackedWeights, few_rows_plan, many_rows_cut
 from packed_models import PackedReferenceKernels
+
+
+def smem_kb(wide, group, columns):
+    """Shared memory of a CTA of the kernel for few rows, by its layout: rings, x, sums, the rows' notes and barriers."""
+    def kb(tokens, warps, splits, batch, depth, run):
+        plane = -(-(-(-columns // 128)) // splits) * 4 * tokens * 64
+        stage = -(-run * (2048 + 128 // group * 64) // 128) * 128
+        return -(-(warps * depth * stage + (2 if wide else 1) * plane + batch * warps * (1024 if tokens <= 8 else 2048) + 128
+                   + warps * depth * 8) // 1024)
+    return kb
+
+
+def plan_of(rows, columns, paired, m, wide=False, group=64, clusters=lambda tokens, warps, splits, kb: 148 // splits):
+    return few_rows_plan(rows, columns, paired, m, wide, smem_kb(wide, group, columns), clusters, 148)
 
 
 def bare_kernels():
@@ -85,3 +100,51 @@ def test_groups_are_whole_numbers_of_the_list(monkeypatch, group):
     if group is not None:
         with pytest.raises(ValueError, match="weight_group"):
             make_runtime("bfloat16", "cpu", kernels=PackedReferenceKernels(), weight_group=group)
+
+
+CLUSTER_SIZES = [(1, 1), (64, 4096), (100, 20000), (64, 65536), (2051, 1021), (4096, 4096), (4096, 12288), (151936, 4096)]
+
+
+@pytest.mark.parametrize("rows,columns", CLUSTER_SIZES)
+@pytest.mark.parametrize("m", [1, 2, 8, 16, 17, 300])
+@pytest.mark.parametrize("paired,wide", [(False, False), (True, False), (False, True)])
+def test_clusters_that_do_not_run_are_no_plan(rows, columns, m, paired, wide):
+    """A device that takes no clusters (or none of 8): a plan keeps to what runs, or there is none."""
+    for largest in (1, 4):
+        p = plan_of(rows, columns, paired, m, wide, clusters=lambda tokens, warps, splits, kb: 148 // splits if splits <= largest else 0)
+        whole = plan_of(rows, columns, paired, m, wide)
+        assert p is None or p.splits <= largest
+        # nothing fits only where x of one row is beyond what CTAs of such clusters hold
+        if p is None:
+            assert whole.splits > largest and smem_kb(wide, 64, columns)(1, 8, largest, 1, 1, 1) > 226
+    assert plan_of(rows, columns, paired, m, wide, clusters=lambda *cut: 0) is None
+
+
+def test_a_device_that_runs_nothing_has_no_cut_for_many_rows():
+    assert many_rows_cut(4096, 4096, False, 200, lambda splits: 0) is None
+    assert many_rows_cut(4096, 4096, False, 20, lambda splits: 74 if splits == 2 else 0).splits == 2
+
+
+def test_a_query_that_failed_is_asked_again(monkeypatch):
+    """What the device says about clusters is kept, but not an error, and no plan that came of one."""
+    class Library:
+        answers = {"few": 0, "many": 0}
+
+        def chibi_packed_few_rows_kb(self, x32, group, columns, *cut):
+            return smem_kb(bool(x32), group, columns)(*cut)
+
+        def chibi_packed_few_rows_clusters(self, x32, group, tokens, warps, splits, kb):
+            return self.answers["few"] // splits
+
+        def chibi_packed_many_rows_clusters(self, splits):
+            return self.answers["many"] // splits
+
+    monkeypatch.setattr(ops, "_PACKED_CLUSTERS", {})
+    k = bare_kernels()
+    k.lib, k.sm_count, k._packed_plans, k._packed_cuts = Library(), 148, {}, {}
+    w = PackedWeights(torch.zeros(1, dtype=torch.uint8), 64, 4096, 64, False)
+    for ask, which in ((lambda: k.packed_plan(w, 1, False), "few"), (lambda: k.packed_cut(w, 200), "many")):
+        with pytest.raises(KernelError):
+            ask()
+        Library.answers[which] = 148
+        assert ask().clusters >= 1
