@@ -821,9 +821,8 @@ CHIBI_API int chibi_packed_few_rows(const ChibiPackedCall* c, const void* x, lon
         return CHIBI_ERR_ARGUMENT;
     const bool x32 = c->x_type == CHIBI_F32;
     const size_t smem = few_rows_smem(x32, c->group, chunks, c->warps, c->splits, c->batch, c->depth, c->run, c->tokens);
-    const long long token_blocks = ((long long)c->m + c->tokens - 1) / c->tokens;
     const int each = c->pair ? PACKED_ROWS / 2 : PACKED_ROWS, row_blocks = (c->n + each - 1) / each;
-    if (smem > FEW_SMEM_LIMIT || token_blocks > 65535)
+    if (smem > FEW_SMEM_LIMIT)
         return CHIBI_ERR_UNSUPPORTED;
     CUtensorMap map;
     memcpy(&map, c->map, sizeof(map));
@@ -833,18 +832,27 @@ CHIBI_API int chibi_packed_few_rows(const ChibiPackedCall* c, const void* x, lon
     while ((1 << along_shift) < c->along_k)
         ++along_shift;
     const int per_unit = c->warps >> along_shift;
-    const FewRows p { row_blocks, chunks, c->n, c->k, c->pair, x, x_stride, c->m, out, c->out_type, out_stride, (const float*)residual,
-                      residual_stride, c->act, c->warps, split_shift, along_shift, c->batch, c->depth, c->run, c->tokens, c->clusters,
-                      (row_blocks + per_unit - 1) / per_unit, (int*)c->error };
+    FewRows p { row_blocks, chunks, c->n, c->k, c->pair, x, x_stride, c->m, out, c->out_type, out_stride, (const float*)residual,
+                residual_stride, c->act, c->warps, split_shift, along_shift, c->batch, c->depth, c->run, c->tokens, c->clusters,
+                (row_blocks + per_unit - 1) / per_unit, (int*)c->error };
     void (*kernel)(const CUtensorMap, const FewRows) = few_rows_kernel(x32, c->tokens, c->group);
     static std::atomic<unsigned long long> allowed[2][2][3];
     const cudaError_t e = packed_allow_shared(kernel, allowed[x32][c->tokens <= 8][c->group / 64], FEW_SMEM_LIMIT);
     if (e != cudaSuccess)
         return (int)e;
-    const dim3 grid((unsigned)(c->clusters * c->splits), (unsigned)token_blocks), block((unsigned)c->warps * 32);
-    if (c->splits > 1)
-        launch_cluster_x(kernel, grid, block, smem, (cudaStream_t)stream, c->splits, map, p);
-    else
-        launch(kernel, grid, block, smem, (cudaStream_t)stream, map, p);
+    const dim3 block((unsigned)c->warps * 32);
+    // (a grid's second axis has 65,535 places: rows of x beyond that many blocks of them are launches of their own)
+    const long long at_once = 65535ll * c->tokens;
+    for (long long first = 0; first < c->m; first += at_once) {
+        p.m = (int)(c->m - first < at_once ? c->m - first : at_once);
+        p.x = static_cast<const char*>(x) + first * x_stride * (x32 ? 4 : 2);
+        p.out = static_cast<char*>(out) + first * out_stride * (c->out_type == CHIBI_F32 ? 4 : 2);
+        p.residual = residual ? static_cast<const float*>(residual) + first * residual_stride : nullptr;
+        const dim3 grid((unsigned)(c->clusters * c->splits), (unsigned)((p.m + c->tokens - 1) / c->tokens));
+        if (c->splits > 1)
+            launch_cluster_x(kernel, grid, block, smem, (cudaStream_t)stream, c->splits, map, p);
+        else
+            launch(kernel, grid, block, smem, (cudaStream_t)stream, map, p);
+    }
     return launch_status();
 }

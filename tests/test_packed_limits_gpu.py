@@ -45,3 +45,29 @@ def test_values_read_back_are_the_next_products_matrix(kernels, m):
         kernels.linear(x, values, out)
         got = out.clone()
         assert torch.equal(got, want[turn % 4]), turn
+
+
+def test_more_rows_of_x_than_a_grid_takes(kernels):
+    """The second axis of a grid ends at 65,535 blocks of 16 rows: more 32-bit rows than that, and bfloat16 ones off 16 bytes."""
+    g = gen(51)
+    w = matrix(g, 8, 9, BF16)
+    packed, pair = kernels.pack_weights(w, 32), kernels.pack_gate_up(w, w.flip(0).contiguous(), 32)
+    values, other = packed_values(w, 32), packed_values(w.flip(0), 32)
+    m = 65535 * 16 + 1000
+    for dtype in (F32, BF16):
+        x = torch.randn(m, 9, generator=g, device=DEV).to(dtype)
+        out = torch.full((m, 8), math.nan, device=DEV)
+        add = torch.randn(m, 8, generator=g, device=DEV)
+        kernels.linear(x, packed, out, residual=add)
+        product = x.double() @ values.t()
+        want = product + add.double()
+        close(out, want, off_by(x, values, 32, F32, product) + want.abs() * 2.0 ** -23)
+        gated = torch.full((m, 8), math.nan, device=DEV)
+        kernels.linear_swiglu(x, pair, gated)
+        up = x.double() @ other.t()
+        want = product * torch.sigmoid(product) * up
+        # (as test_gated_pairs has it)
+        a, b = off_by(x, values, 32, F32, product), off_by(x, other, 32, F32, up)
+        bound = (1.13 * a + 8 * 2.0 ** -24 * product.abs()) * (up.abs() + b) + product.abs() * b + want.abs() * 2.0 ** -24 + 1e-30
+        close(gated, want, bound)
+    kernels.check_error_word()
