@@ -505,7 +505,7 @@ CHIBI_API int chibi_packed_many_rows_clusters(int splits)
 
 // out[m, n] = x[m, k] times the matrix (+ residual); pair: act(x gate) * (x up), n features.  `tokens`: rows of x of a tile;
 // every CTA takes `rounds` whole tiles, what is left is shared by clusters of `splits` CTAs, `clusters` of them (splits 1: CTAs).
-// CHIBI_ERR_UNSUPPORTED where x's rows do not start on 16 bytes.
+// CHIBI_ERR_UNSUPPORTED where x's rows do not start on 16 bytes, or overlap (a tensor map's strides are at least its rows).
 CHIBI_API int chibi_packed_many_rows(const ChibiPackedCall* c, const void* x, long long x_stride, void* out, long long out_stride,
                                      const void* residual, long long residual_stride, void* stream)
 {
@@ -515,7 +515,7 @@ CHIBI_API int chibi_packed_many_rows(const ChibiPackedCall* c, const void* x, lo
     const int chunks = (c->k + PACKED_COLS - 1) / PACKED_COLS, tokens = c->tokens, splits = c->splits;
     if ((tokens != 48 && tokens != 96 && tokens != 192) || splits < 1 || splits > 8 || splits > chunks || c->rounds < 0 || c->clusters < 1)
         return CHIBI_ERR_ARGUMENT;
-    if ((reinterpret_cast<uintptr_t>(x) & 15) || x_stride % 8)
+    if ((reinterpret_cast<uintptr_t>(x) & 15) || x_stride % 8 || x_stride < c->k)
         return CHIBI_ERR_UNSUPPORTED;
     const int tile_rows = c->pair ? PT_ROWS / 2 : PT_ROWS;
     const long long token_tiles = (c->m + (long long)tokens - 1) / tokens, tiles = (c->n + (long long)tile_rows - 1) / tile_rows * token_tiles;

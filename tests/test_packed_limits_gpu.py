@@ -71,3 +71,18 @@ def test_more_rows_of_x_than_a_grid_takes(kernels):
         bound = (1.13 * a + 8 * 2.0 ** -24 * product.abs()) * (up.abs() + b) + product.abs() * b + want.abs() * 2.0 ** -24 + 1e-30
         close(gated, want, bound)
     kernels.check_error_word()
+
+
+@pytest.mark.parametrize("m", [5, 40, 300])
+def test_rows_of_x_that_overlap(kernels, m):
+    """One row for all (an expanded tensor), and rows that begin within the row before: what no tile copy is described for."""
+    g = gen(52)
+    w = matrix(g, 200, 256, BF16)
+    packed, values = kernels.pack_weights(w, 64), packed_values(w, 64)
+    line = torch.randn(8 * m + 256, generator=g, device=DEV).to(BF16)
+    for x in (line[:256].expand(m, 256), line.as_strided((m, 256), (8, 1)), line.as_strided((m, 256), (3, 1))):
+        out = torch.empty(m, 200, device=DEV)
+        kernels.linear(x, packed, out)
+        want = x.double() @ values.t()
+        close(out, want, off_by(x, values, 64, F32, want))
+    kernels.check_error_word()
