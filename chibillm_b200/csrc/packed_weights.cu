@@ -288,11 +288,15 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // multiplied by the scales in 32 bits.
 //
 // x becomes float16 too (two nibbles of a word are float16 numbers without a shift, which bfloat16's seven bits of mantissa
-// do not allow; the conversion of the codes is most of the kernel's instructions).  A row of bfloat16 whose largest number of the CTA's
-// columns is not within 1 ... 2^15, and every row of 32-bit numbers, is multiplied by the power of two that brings the largest to
-// 2^14 ... 2^15, and its sums by the inverse.  So bfloat16 numbers from 2^-14 (of a scaled row: 2^-29 of the largest) on keep all of their
-// bits, smaller ones are off by 2^-25 (2^-40) at most.  32-bit numbers are two float16 numbers, the nearest and the nearest to what is
-// left: off by 2^-23 of themselves or by 2^-40 of the row's largest at most, no more than the 32-bit sums lose.
+// do not allow; the conversion of the codes is most of the kernel's instructions).  A row's numbers, as far as the CTA's columns go, are
+// multiplied by a power of two and its sums by the inverse: 2^6 where that keeps every bit of a bfloat16 row (its numbers within
+// 2^-20 ... 2^9, as a norm's output has them, or zero), else the one that brings the largest to 2^14 ... 2^15.  So bfloat16 numbers from
+// 2^-28 of the largest on keep all of their bits.  32-bit numbers are two float16 numbers, the nearest and the nearest to what is left:
+// off by 2^-23 of themselves, or by 2^-25, half of float16's last step, which is 2^-39 of the row's largest at most and 2^-16 of
+// numbers from 2^-9 on.  What is smaller (bfloat16: 2^-14, 32-bit: 2^-9, as multiplied) and lost bits is added to the warps' sums in
+// 32 bits after the stream, so nothing vanishes beside a large number whose weights are zeros (add_what_was_lost; a row of 4,096 normal
+// numbers has one with a chance of 1e-5, a 32-bit one of 1e-3; one such number makes the product with 4,096 x 4,096 take 6.8 us
+// instead of 4.8, a row of nothing else 30).
 //
 // How the work is shared out (CudaKernels.packed_plan chooses): `splits` CTAs of a cluster share the columns, `along_k`
 // warps of a CTA share the CTA's columns of one block of 32 rows, the CTA's warps / along_k blocks of rows are a unit, and clusters
@@ -320,6 +324,7 @@ struct FewRows {
     int warps, split_shift, along_shift, batch, depth, run, tokens;  // run: records of a stage; tokens: rows of x of a CTA
     int clusters, units;
     int* error;
+    const uint8_t* data;           // the records, for what goes around the tile copies
 };
 
 // FIRST: d is what comes out, else it is added to.
@@ -343,12 +348,13 @@ __device__ __forceinline__ float peer_shared_f32(uint32_t own_smem_addr, uint32_
     return v;
 }
 
-// The exponent of the power of two by which a row is multiplied, from its largest finite magnitude: the one that brings it to
-// 2^14 ... 2^15 (as far as a 32-bit number goes: rows below 2^-112 come out smaller), for bfloat16 none where it is 1 ... 2^15.
-template <bool X32> __device__ __forceinline__ int row_exponent(uint32_t largest_bits)
+// The exponents of the powers of two by which rows are multiplied: the first, with the range that it suits (as bits of an exponent),
+// and what a row's largest finite magnitude asks for.  (As far as a 32-bit number goes: rows below 2^-112 come out smaller.)
+constexpr int ROW_EXPONENT = 6;
+constexpr uint32_t ROW_LEAST = 127 - 14 - ROW_EXPONENT, ROW_MOST = 127 + 15 - ROW_EXPONENT;
+__device__ __forceinline__ int row_exponent(uint32_t largest_bits)
 {
-    const int e = (int)(largest_bits >> 23) - 127;
-    return (!X32 && e >= 0 && e < 15) || largest_bits == 0 ? 0 : min(14 - e, 126);
+    return largest_bits == 0 ? 0 : min(14 + 127 - (int)(largest_bits >> 23), 126);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -361,8 +367,68 @@ __device__ __forceinline__ uint32_t take_half_pair(float (&v)[2])
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Numbers below this, as multiplied, may have lost bits that count.
+template <bool X32> __device__ __forceinline__ float least_kept() { return X32 ? 0x1p-9f : 0x1p-14f; }
+// What float16 has lost of such a number, exactly: v and the multiple of 2^(-24 - e) next to it differ by what 24 bits hold.
+template <bool X32> __device__ __forceinline__ float lost_of(float v, int e)
+{
+    const float up = v * power_of_two(e);
+    float held = __half2float(__float2half_rn(up));
+    if (X32)
+        held += __half2float(__float2half_rn(up - held));
+    return fabsf(up) < least_kept<X32>() ? fmaf(-held, power_of_two(-e), v) : 0.f;
+}
+
+// Adds what the rows of x in `rows` (a bit each) lost to a warp's sums of a block of 32 rows of the matrix, columns w0 ... w1: a
+// lane a row of the matrix.  A number that lost nothing costs its test alone, 32 columns at a time.
+template <bool X32, int NT>
+__device__ __noinline__ void add_what_was_lost(const FewRows& p, uint32_t rows, int token0, int block, int w0, int w1, int group,
+                                               const uint32_t* largest, float* sums)
+{
+    using T = typename std::conditional<X32, float, __nv_bfloat16>::type;
+    const int lane = threadIdx.x & 31;
+    for (; rows != 0; rows &= rows - 1) {
+        const int token = __ffs(rows) - 1;
+        const T* x = static_cast<const T*>(p.x) + (token0 + token) * p.x_stride;
+        const int e = row_exponent(largest[token]);
+        float sum = 0.f;
+#pragma unroll 1
+        for (int chunk = w0; chunk < w1; ++chunk) {
+            float lost[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {                    // blocks of 32 columns
+                const int col = chunk * PACKED_COLS + b * 32 + lane;
+                lost[b] = col < p.k ? to_f32(x[col]) : 0.f;
+            }
+            bool any = false;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                lost[b] = lost_of<X32>(lost[b], e);
+                any = any || lost[b] != 0.f;
+            }
+            if (!__any_sync(0xffffffffu, any))
+                continue;
+            const uint8_t* rec = p.data + ((long long)block * p.chunks + chunk) * packed_record_bytes(group);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float part = 0.f;
+#pragma unroll 1
+                for (uint32_t todo = __ballot_sync(0xffffffffu, lost[b] != 0.f); todo != 0; todo &= todo - 1) {
+                    const int j = __ffs(todo) - 1;
+                    const uint32_t word = *reinterpret_cast<const uint32_t*>(rec + packed_word_at(lane, b * 4 + (j >> 3)));
+                    const int q = (int)((word >> (4 * ((j & 7) / 2) + 16 * (j & 1))) & 15u) - 8;
+                    part = fmaf((float)q, __shfl_sync(0xffffffffu, lost[b], j), part);
+                }
+                sum = fmaf(to_f32(*reinterpret_cast<const __nv_bfloat16*>(rec + packed_scale_at(lane, b * 32 / group))), part, sum);
+            }
+        }
+        // (the fragment's place of the row and the token)
+        sums[(((lane >> 4) * NT + (token >> 3)) * 4 + ((lane >> 3) & 1) * 2 + (token & 1)) * 32 + (lane & 7) * 4 + (token & 7) / 2] += sum;
+    }
+}
+
 template <int NT, bool X32, int GROUP_BLOCKS>
-__global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const __grid_constant__ CUtensorMap map, const FewRows p)
+__global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ FewRows p)
 {
     using namespace sm100;
     using T = typename std::conditional<X32, float, __nv_bfloat16>::type;
@@ -384,14 +450,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     const int most = (p.chunks + splits - 1) >> p.split_shift;
     const int unit_shift = (p.warps == 16 ? 4 : 3) - p.along_shift, blocks_per_unit = 1 << unit_shift;
 
-    // shared memory: rings | x | sums | the rows' largest numbers | barriers
+    // shared memory: rings | x | sums | the rows' largest numbers, a bit for each that lost bits | barriers
     const uint32_t x_plane = (uint32_t)most * 4 * p.tokens * 64;
     const int stage = (p.run * RECORD + 127) / 128 * 128;        // (a tile copy's place starts on 128 bytes)
     uint8_t* ring = smem + warp * p.depth * stage;
     uint8_t* xs = smem + p.warps * p.depth * stage;
     float* sums = reinterpret_cast<float*>(xs + (size_t)PARTS * x_plane);
     uint32_t* largest = reinterpret_cast<uint32_t*>(sums + p.batch * p.warps * SUMS);
-    uint64_t* full = reinterpret_cast<uint64_t*>(largest + 16) + warp * p.depth;
+    uint64_t* full = reinterpret_cast<uint64_t*>(largest + 18) + warp * p.depth;
 
     // the warp's records: of its block of rows in every unit, columns w0 ... w1
     const int wk = warp & (along_k - 1), wr = warp >> p.along_shift;
@@ -416,7 +482,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     if (lane == 0)
         for (int i = 0; i < p.depth; ++i)
             mbar_init(&full[i], 1);
-    if (threadIdx.x < 16)
+    if (threadIdx.x < 18)
         largest[threadIdx.x] = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -444,14 +510,25 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
             *reinterpret_cast<uint4*>(dst + part * x_plane)
                 = make_uint4(take_half_pair(pairs[0]), take_half_pair(pairs[1]), take_half_pair(pairs[2]), take_half_pair(pairs[3]));
     };
-    // bfloat16 rows once as they are, and those that want a factor once more; 32-bit rows when the factor is known
+    // 32-bit rows are looked at first.  bfloat16 rows are multiplied by 2^6 at once, and only if a CTA has a number that this does not suit
+    // (two at a time, their bits as whole numbers; less 1, so that a zero is the largest of all) are its rows looked at and what has
+    // to be is done once more.
+    constexpr float AT_FIRST = float(1 << ROW_EXPONENT);
+    uint32_t most_two = 0, least_two = 0xffffffffu;
+    auto put_at_first = [&](int i, const T (&raw)[8]) {
+        put(i, raw, AT_FIRST);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t two = reinterpret_cast<const uint32_t*>(raw)[j] & 0x7fff7fffu;
+            most_two = __vmaxu2(most_two, two);
+            least_two = __viaddmin_u16x2(two, 0xffffffffu, least_two);
+        }
+    };
     float most_of = 0.f;
     auto look = [&](const T (&raw)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float v = fabsf(to_f32(raw[j]));
-            most_of = v < INFINITY ? fmaxf(most_of, v) : most_of;
-        }
+        for (int j = 0; j < 8; ++j)
+            most_of = fmaxf(most_of, fabsf(to_f32(raw[j])));
     };
     if (((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)p.x_stride * sizeof(T)) & 15) == 0 && (p.k & 7) == 0) {
         // whole pieces on 16 bytes
@@ -470,9 +547,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
             // (one copy of the code for all of them: what a kernel runs once it waits for)
 #pragma unroll 1
             for (int i = i0; i < min(i0 + AT_ONCE * step, token_pieces); i += step) {
-                look(raw[0]);
-                if constexpr (!X32)
-                    put(i, raw[0], 1.f);
+                if constexpr (X32)
+                    look(raw[0]);
+                else
+                    put_at_first(i, raw[0]);
 #pragma unroll
                 for (int a = 0; a + 1 < AT_ONCE; ++a)
 #pragma unroll
@@ -483,26 +561,57 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     } else {
 #pragma unroll 1
         for (int i = first_piece; i < token_pieces; i += step) {
-            T raw[8];
+            __align__(16) T raw[8];
             read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
-            look(raw);
-            if constexpr (!X32)
-                put(i, raw, 1.f);
+            if constexpr (X32)
+                look(raw);
+            else
+                put_at_first(i, raw);
         }
     }
-    const uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
-    if (lane == 0)
-        atomicMax(&largest[token], warps_most);
-    __syncthreads();
-    if (const int e = row_exponent<X32>(largest[token]); X32 || e != 0) {
+    bool looked_at = true;
+    if constexpr (!X32) {
+        looked_at = __syncthreads_or(max(most_two >> 16, most_two & 0xffffu) >= ROW_MOST << 7 || min(least_two >> 16, least_two & 0xffffu) < (ROW_LEAST << 7) - 1);
+        if (__builtin_expect(looked_at, false))
+#pragma unroll 1
+            for (int i = first_piece; i < token_pieces; i += step) {
+                __align__(16) T raw[8];
+                read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
+                look(raw);
+            }
+    }
+    if (__builtin_expect(looked_at, X32)) {
+        uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
+        if (warps_most == 0x7f800000u) {         // (an infinity: the largest of the others; fmaxf passes NaN over)
+            most_of = 0.f;
+#pragma unroll 1
+            for (int i = first_piece; i < token_pieces; i += step) {
+                __align__(16) T raw[8];
+                read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    most_of = fabsf(to_f32(raw[j])) < INFINITY ? fmaxf(most_of, fabsf(to_f32(raw[j]))) : most_of;
+            }
+            warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
+        }
+        if (lane == 0)
+            atomicMax(&largest[token], warps_most);
+        __syncthreads();
+        const int e = row_exponent(largest[token]);
+        uint32_t smallest = 0xffffffffu;         // but zero, its bits less 1
 #pragma unroll 1
         for (int i = first_piece; i < token_pieces; i += step) {
-            T raw[8];
+            __align__(16) T raw[8];
             read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
             put(i, raw, power_of_two(e));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                smallest = __viaddmin_u32(__float_as_uint(to_f32(raw[j])) & 0x7fffffffu, 0xffffffffu, smallest);
         }
+        if (smallest < __float_as_uint(least_kept<X32>() * power_of_two(-e)) - 1)
+            atomicOr(&largest[16], 1u << token);
+        __syncthreads();
     }
-    __syncthreads();
 
     // ---- the stream
     const int r = lane >> 2, c = lane & 3;
@@ -514,7 +623,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
         x_lane[t] = (uint32_t)min(t * 8 + r, tokens - 1) * 64 + c * 16;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            down[t][j] = power_of_two(-row_exponent<X32>(largest[min(t * 8 + 2 * c + j, tokens - 1)]));
+            down[t][j] = 1.f / AT_FIRST;
+    }
+    uint32_t lossy = 0;                          // the rows with numbers that lost bits
+    if (__builtin_expect(looked_at, X32)) {
+        lossy = largest[16];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                down[t][j] = power_of_two(-row_exponent(largest[min(t * 8 + 2 * c + j, tokens - 1)]));
     }
     const uint32_t x_block = (uint32_t)p.tokens * 64;
     bool dead = false;                           // a wait ran out: nothing more is asked for
@@ -610,6 +728,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
                     for (int e = 0; e < 4; ++e)
                         mine[((h * NT + t) * 4 + e) * 32] = acc[h][t][e] * down[t][e & 1];
         }
+        if (__builtin_expect(lossy != 0, false)) {
+            __syncwarp();
+            for (int u = 0; u < min(now, warp_rounds - first); ++u)
+                add_what_was_lost<X32, NT>(p, lossy, token0, (cluster + (first + u) * p.clusters) * blocks_per_unit + wr, w0, w1,
+                                           GROUP_BLOCKS * 32, largest, sums + (u * p.warps + warp) * SUMS);
+        }
 
         // ---- the cluster adds up what its warps have
         __syncthreads();
@@ -686,7 +810,7 @@ size_t few_rows_smem(bool x32, int group, int chunks, int warps, int splits, int
 {
     const size_t x_plane = (size_t)((chunks + splits - 1) / splits) * 4 * tokens * 64;
     return (size_t)warps * depth * ((run * packed_record_bytes(group) + 127) / 128 * 128) + (x32 ? 2 : 1) * x_plane
-        + (size_t)batch * warps * 256 * (tokens <= 8 ? 1 : 2) * 4 + 16 * 4 + warps * depth * 8;
+        + (size_t)batch * warps * 256 * (tokens <= 8 ? 1 : 2) * 4 + 18 * 4 + warps * depth * 8;
 }
 
 void (*few_rows_kernel(bool x32, int tokens, int group))(const CUtensorMap, const FewRows)
@@ -834,7 +958,8 @@ CHIBI_API int chibi_packed_few_rows(const ChibiPackedCall* c, const void* x, lon
     const int per_unit = c->warps >> along_shift;
     FewRows p { row_blocks, chunks, c->n, c->k, c->pair, x, x_stride, c->m, out, c->out_type, out_stride, (const float*)residual,
                 residual_stride, c->act, c->warps, split_shift, along_shift, c->batch, c->depth, c->run, c->tokens, c->clusters,
-                (row_blocks + per_unit - 1) / per_unit, (int*)c->error };
+                (row_blocks + per_unit - 1) / per_unit, (int*)c->error,
+                static_cast<const uint8_t*>(c->data) };
     void (*kernel)(const CUtensorMap, const FewRows) = few_rows_kernel(x32, c->tokens, c->group);
     static std::atomic<unsigned long long> allowed[2][2][3];
     const cudaError_t e = packed_allow_shared(kernel, allowed[x32][c->tokens <= 8][c->group / 64], FEW_SMEM_LIMIT);

@@ -86,3 +86,62 @@ def test_rows_of_x_that_overlap(kernels, m):
         want = x.double() @ values.t()
         close(out, want, off_by(x, values, 64, F32, want))
     kernels.check_error_word()
+
+
+def whole_numbers(g, m, n, k, group, x_dtype):
+    """Codes, scales that are powers of two and x of small whole numbers: every sum is exact in 32 bits in any order
+    (k * 8 * 15 * 2^3 < 2^24 steps)."""
+    codes = torch.randint(-8, 8, (n, k), generator=g, device=DEV, dtype=torch.int8)
+    scales = (2.0 ** torch.randint(-3, 1, (n, -(-k // group)), generator=g, device=DEV)).to(BF16)
+    x = torch.randint(-15, 16, (m, k), generator=g, device=DEV).to(x_dtype)
+    return codes, scales, x
+
+
+def values_of(codes, scales, group):
+    return codes.double() * scales.double().repeat_interleave(group, 1)[:, :codes.shape[1]]
+
+
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(1, 70, 200), (3, 2048, 1024), (8, 33, 4096), (11, 300, 1021), (16, 64, 2048), (1, 32, 8192)])
+def test_numbers_of_all_sizes_in_one_row(kernels, m, n, k, group, x_dtype):
+    """A large number that meets only zeros leaves no trace, however small the others are."""
+    g = gen(53 + m)
+    codes, scales, x = whole_numbers(g, m, n, k, group, x_dtype)
+    at = [0, k // 2, k - 1]
+    codes[:, at] = 0
+    packed = kernels.pack_codes(codes, scales, group)
+    values = values_of(codes, scales, group)
+    out = torch.empty(m, n, device=DEV)
+    for small in (1.0, 2.0 ** -8, 2.0 ** -20, 2.0 ** -40, 2.0 ** -100):
+        for large in (2.0 ** 9, 2.0 ** 20, 2.0 ** 50, 2.0 ** 126):
+            rows = x * small
+            rows[:, at] = large
+            if m > 1:
+                rows[1, at[1:]] = 0.0              # (a row of its own range)
+            want = rows.double() @ values.t()
+            kernels.linear(rows, packed, out)
+            assert torch.equal(out.double(), want), (small, large)
+    kernels.check_error_word()
+
+
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 4096), (4, 64, 20000), (16, 100, 1000)])
+def test_rows_whose_sizes_run_from_the_smallest_to_the_largest(kernels, m, n, k, x_dtype):
+    """Whatever part of a row a column of the matrix sees, its numbers have kept their bits: bfloat16 all of them, 32-bit ones all
+    but 2^-23 of themselves, and 2^-16 where they are below 2^-16 of the row's largest (a float16's last half step, 2^-25,
+    against numbers from 2^-9 on, multiplied so that the row's largest is 2^14 ... 2^15; smaller numbers are added apart)."""
+    g = gen(54 + m)
+    x = torch.randn(m, k, generator=g, device=DEV, dtype=torch.float64) * 2.0 ** torch.linspace(-100, 100, k, device=DEV, dtype=torch.float64)
+    x = x.to(x_dtype)
+    codes = torch.zeros(n, k, dtype=torch.int8, device=DEV)
+    scales = torch.ones(n, -(-k // 32), dtype=BF16, device=DEV)
+    start = torch.linspace(0, k - 8, n, device=DEV).long()
+    for j in range(8):                             # row i of the matrix sees 8 neighbouring columns
+        codes[torch.arange(n, device=DEV), start + j] = torch.randint(1, 8, (n,), generator=g, device=DEV, dtype=torch.int8)
+    packed, values = kernels.pack_codes(codes, scales, 32), values_of(codes, scales, 32)
+    out = torch.empty(m, n, device=DEV)
+    kernels.linear(x, packed, out)
+    want = x.double() @ values.t()
+    own = (x.double().abs() @ values.t()) * (2.0 ** -16 if x_dtype == F32 else 0.0)
+    close(out, want, off_by(x, values, 32, F32, want) + own)
