@@ -125,4 +125,59 @@ template <bool ROUNDED> __device__ __forceinline__ float packed_activate(float z
     return ROUNDED ? __fdividef(z, 1.f + __expf(-y)) : z / (1.f + expf(-y));
 }
 
+// 8 neighbouring numbers of a row from column `col` on, zeros beyond its k columns.
+template <typename T> __device__ __forceinline__ void read_eight(const T* row, int col, int k, T (&v)[8])
+{
+    const T* src = row + col;
+    if (col + 8 <= k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = col + i < k ? src[i] : from_f32<T>(0.f);
+    }
+}
+
+// Products of rows of the matrix with rows of x, by a warp each and in 64 bits: for sums that came out as no number although every
+// number of x is one (a group's sum, or its product with a scale, can pass 2^128 where the whole does not: weights from 10^32 on,
+// x from 10^35 on).  Terms are exact (4, 8 and 24 bits).  The whole warp calls; a lane that asks has the block of rows, the row in
+// its records and the row of x, and gets the sum instead of v.  Slow, 6 us for 4,096 columns (less where a NaN ends it).
+template <typename T>
+__device__ __forceinline__ float packed_sums_in_64_bits(const uint8_t* data, int group, int chunks, int k, bool asks, int block, int r,
+                                                        const T* x, float v)
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (uint32_t todo = __ballot_sync(0xffffffffu, asks); todo != 0; todo &= todo - 1) {
+        const int who = __ffs(todo) - 1;
+        const int row = __shfl_sync(0xffffffffu, r, who);
+        const uint8_t* rec = data + (long long)__shfl_sync(0xffffffffu, block, who) * chunks * packed_record_bytes(group);
+        const T* from = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(x), who));
+        double sum = 0.;
+#pragma unroll 1
+        for (int col = lane * 8; __any_sync(0xffffffffu, col < k); col += 256) {
+            if (col < k) {
+                __align__(16) T eight[8];
+                read_eight(from, col, k, eight);
+                const uint8_t* at = rec + (long long)(col / PACKED_COLS) * packed_record_bytes(group);
+                const uint32_t word = *reinterpret_cast<const uint32_t*>(at + packed_word_at(row, col % PACKED_COLS >> 3));
+                double part = 0.;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    part = fma((double)((int)((word >> (4 * (i / 2) + 16 * (i & 1))) & 15u) - 8), (double)to_f32(eight[i]), part);
+                sum = fma((double)to_f32(*reinterpret_cast<const __nv_bfloat16*>(at + packed_scale_at(row, col % PACKED_COLS / group))), part, sum);
+            }
+            if (__any_sync(0xffffffffu, sum != sum))
+                break;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        v = lane == who ? (float)sum : v;
+    }
+    return v;
+}
+
 } // namespace chibi

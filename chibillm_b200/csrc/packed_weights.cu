@@ -70,21 +70,6 @@ template <typename T> __device__ __forceinline__ uint32_t code_word(const T (&w)
     return word;
 }
 
-// 8 neighbouring numbers of a row from column `col` on, zeros beyond its k columns.
-template <typename T> __device__ __forceinline__ void read_eight(const T* row, int col, int k, T (&v)[8])
-{
-    const T* src = row + col;
-    if (col + 8 <= k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-            reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = col + i < k ? src[i] : from_f32<T>(0.f);
-    }
-}
-
 // Products fetch their matrix before the kernel ahead of them has ended.  So the kernels that write one, in 4 bits or as values read
 // back, let nothing start early (no pdl_trigger; and no mark in a timeline), and every thread's stores are performed, for tile copies
 // too, before it ends.
@@ -427,6 +412,18 @@ __device__ __noinline__ void add_what_was_lost(const FewRows& p, uint32_t rows, 
     }
 }
 
+// (v, up) with the sums in 64 bits where they are no numbers (packed_sums_in_64_bits).
+template <bool X32>
+__device__ __noinline__ float2 sums_in_64_bits(const FewRows& p, int group, bool there, int block, int r, int m, float2 v)
+{
+    using T = typename std::conditional<X32, float, __nv_bfloat16>::type;
+    const T* x = static_cast<const T*>(p.x) + m * p.x_stride;
+    v.x = packed_sums_in_64_bits(p.data, group, p.chunks, p.k, there && !isfinite(v.x), block, r, x, v.x);
+    if (p.pair)
+        v.y = packed_sums_in_64_bits(p.data, group, p.chunks, p.k, there && !isfinite(v.y), block, r + 8, x, v.y);
+    return v;
+}
+
 template <int NT, bool X32, int GROUP_BLOCKS>
 __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ FewRows p)
 {
@@ -752,13 +749,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
         }
         const int rows_out = p.pair ? PACKED_ROWS / 2 : PACKED_ROWS;
         const int outputs = now * blocks_per_unit * rows_out * tokens;
-        for (int e = rank * blockDim.x + threadIdx.x; e < outputs; e += splits * blockDim.x) {
+        for (int e0 = rank * blockDim.x + warp * 32; e0 < outputs; e0 += splits * blockDim.x) {
+            const int e = min(e0 + lane, outputs - 1);
             const int row = e & (rows_out - 1), rest = e >> (p.pair ? 4 : 5);
             const int block = rest / tokens, token = rest - block * tokens;          // block: of the batch, unit by unit
             const int u = block >> unit_shift, b = block & (blocks_per_unit - 1);
-            const int at = ((cluster + (first + u) * p.clusters) * blocks_per_unit + b) * rows_out + row;
-            if (at >= p.n)
-                continue;
+            const int block_at = (cluster + (first + u) * p.clusters) * blocks_per_unit + b, at = block_at * rows_out + row;
+            const bool there = e0 + lane < outputs && at < p.n;
             // the fragment's place of (row of the record, token); a pair's up lies two registers behind its gate
             const int in_record = p.pair ? (row >> 3) * 16 + (row & 7) : row;
             const int reg = ((in_record >> 4) * NT + (token >> 3)) * 4 + ((in_record >> 3) & 1) * 2 + (token & 1);
@@ -779,6 +776,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
                         up += place[w * SUMS + 64];
                 }
             }
+            // (sums that passed 2^128, or x or a scale that is no number)
+            if (__builtin_expect(__any_sync(0xffffffffu, there && !(fabsf(v) + fabsf(up) < INFINITY)), false)) {
+                const float2 both = sums_in_64_bits<X32>(p, GROUP_BLOCKS * 32, there, block_at, in_record, token0 + token, make_float2(v, up));
+                v = both.x;
+                up = both.y;
+            }
+            if (!there)
+                continue;
             if (p.pair)
                 v = (p.out_type == CHIBI_F32 ? packed_activate<false>(v, p.act) : packed_activate<true>(v, p.act)) * up;
             const long long m = token0 + token;

@@ -145,3 +145,52 @@ def test_rows_whose_sizes_run_from_the_smallest_to_the_largest(kernels, m, n, k,
     want = x.double() @ values.t()
     own = (x.double().abs() @ values.t()) * (2.0 ** -16 if x_dtype == F32 else 0.0)
     close(out, want, off_by(x, values, 32, F32, want) + own)
+
+
+def rows_beyond_32_bits(g, m, n, k, group, x_dtype):
+    """(x, codes, scales): products whose sums are whole numbers, exact in 32 bits, on a way that passes 2^128.  Rows of x in turn:
+    tiny ones that meet huge scales, huge ones that meet tiny scales, huge ones whose terms cancel."""
+    codes = torch.randint(1, 8, (n, k), generator=g, device=DEV, dtype=torch.int8)
+    codes[:, 1::2] = -codes[:, 0:-1:2] if k % 2 == 0 else torch.cat([-codes[:, 0:-1:2]], 1)[:, :codes[:, 1::2].shape[1]]
+    codes[:, :4] = 7
+    groups = -(-k // group)
+    scales = torch.empty(n, groups, dtype=BF16, device=DEV)
+    scales[0::2], scales[1::2] = 2.0 ** 110, 2.0 ** -100
+    x = torch.zeros(m, k, device=DEV)
+    x[0::3, :4] = 2.0 ** -104                     # 28 * 2^6 with the first scale, as multiplied 2^14 * 28 * 2^110
+    x[1::3, :4] = 2.0 ** 120                      # 28 * 2^20 with the second
+    x[2::3] = 2.0 ** 122                          # neighbours cancel: 28 * 2^22 and less with the second
+    return x.to(x_dtype), codes, scales
+
+
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 64), (3, 70, 300), (7, 2048, 1024), (16, 33, 2048), (12, 64, 30000)])
+def test_sums_whose_way_passes_32_bits(kernels, m, n, k, group, x_dtype):
+    g = gen(60 + m)
+    x, codes, scales = rows_beyond_32_bits(g, m, n, k, group, x_dtype)
+    packed, values = kernels.pack_codes(codes, scales, group), values_of(codes, scales, group)
+    out = torch.empty(m, n, device=DEV)
+    for rows in (x, x.flip(0).contiguous()):
+        kernels.linear(rows, packed, out)
+        want = (rows.double() @ values.t()).float()        # (what is beyond 2^128 is infinite)
+        assert want.isfinite().any() and torch.equal(out, want)
+    # what is no number in x stays what it is
+    x[0, k - 1] = math.inf
+    kernels.linear(x, packed, out)
+    want = (x.double() @ values.t()).float()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(0.0), want.nan_to_num(0.0))
+    # a pair: the gate's sum on such a way, up's plain
+    ones = torch.zeros(n, k, dtype=torch.int8, device=DEV)
+    ones[:, 0] = 1
+    x, _, _ = rows_beyond_32_bits(g, m, n, k, group, x_dtype)
+    pair = kernels.pack_codes(codes, scales, group, ones, torch.full_like(scales, 2.0 ** 100))
+    gate, up = (x.double() @ values.t()), x[:, :1].double() * 2.0 ** 100
+    want = gate * torch.sigmoid(gate) * up
+    gated = torch.empty(m, n, device=DEV)
+    kernels.linear_swiglu(x, pair, gated)
+    fits = (gate.abs() < 2.0 ** 127) & (up.abs() < 2.0 ** 127) & (want.abs() < 2.0 ** 127)
+    assert fits.any()
+    # (expf and the division are good to 2 half steps each, the product to one; gate and up are exact)
+    assert ((gated.double() - want).abs() <= want.abs() * 8 * 2.0 ** -24 + 2.0 ** -149)[fits].all()
+    kernels.check_error_word()
