@@ -106,12 +106,15 @@ __device__ __forceinline__ void packed_half_pairs(uint32_t word, uint32_t (&pair
     asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[3]) : "r"(0x2c002c00u), "r"(0xd480d480u));
 }
 
-// The same as bfloat16 (128 + code has its code in the lowest of bfloat16's seven bits of mantissa).
+// The same as bfloat16, times 2^-10 (2^-3 + 2^-10 code has its code in the lowest of bfloat16's seven bits of mantissa).  A group's
+// sum over 128 finite bfloat16 numbers is below 2^138, times 2^-10 within 32 bits; PACKED_BF16_UNDO brings it back.  (Sums of x below
+// 2^-120 come into the range where 32-bit numbers have fewer bits.)
+constexpr float PACKED_BF16_UNDO = 1024.f;
 template <int J> __device__ __forceinline__ uint32_t packed_bf16_pair(uint32_t word)
 {
     uint32_t r;
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(r) : "r"(word >> (4 * J)));
-    asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(r) : "r"(0x43084308u));                           // - 136
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x3e003e00, 0xea;" : "=r"(r) : "r"(word >> (4 * J)));
+    asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(r) : "r"(0x3e083e08u));                           // - 136 * 2^-10
     return r;
 }
 

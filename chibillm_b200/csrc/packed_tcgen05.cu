@@ -6,7 +6,9 @@
 // codes into bfloat16 whole numbers (exact) and write them to TMEM, where they are the A operand: shared memory carries only
 // the rows of x and the codes themselves.  Each group's sum is an accumulator of its own in TMEM; three warpgroups read it, each
 // a third of the columns, and add it times the row's scale to sums in registers.  So nothing is rounded but 32-bit sums, and a
-// lane's row has one scale for all of its columns.  A thread's sums are an output column of 32 lanes: stores are whole
+// lane's row has one scale for all of its columns.  (The whole numbers are held times 2^-10, so that the sums of finite x are
+// finite; a CTA's sums are multiplied by 2^10 in the end.  They are infinite where they pass 2^128, or a group's part of them
+// 2^138.)  A thread's sums are an output column of 32 lanes: stores are whole
 // lines without a detour.
 //
 // What bounds it: an instruction of 128 x TOKENS x 16 with its A operand in TMEM takes 118 cycles at 64 as at 128 columns, so tiles
@@ -375,6 +377,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                 }
             if (!ok)
                 break;
+#pragma unroll
+            for (int j = 0; j < COLS / 2; ++j)
+                acc[j] = pair_mul(acc[j], pair_of(PACKED_BF16_UNDO, PACKED_BF16_UNDO));
             if (r == p.rounds) {
                 // [column][row], where x was: all of this CTA's copies and products are done
                 float* mine = reinterpret_cast<float*>(xs) + part * COLS * PT_ROWS + quarter * 32 + lane;

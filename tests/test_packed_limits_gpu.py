@@ -103,7 +103,8 @@ def values_of(codes, scales, group):
 
 @pytest.mark.parametrize("x_dtype", [BF16, F32])
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("m,n,k", [(1, 70, 200), (3, 2048, 1024), (8, 33, 4096), (11, 300, 1021), (16, 64, 2048), (1, 32, 8192)])
+@pytest.mark.parametrize("m,n,k", [(1, 70, 200), (3, 2048, 1024), (8, 33, 4096), (11, 300, 1021), (16, 64, 2048), (1, 32, 8192),
+                                   (20, 130, 2048), (90, 64, 512), (300, 2050, 264)])
 def test_numbers_of_all_sizes_in_one_row(kernels, m, n, k, group, x_dtype):
     """A large number that meets only zeros leaves no trace, however small the others are."""
     g = gen(53 + m)
@@ -113,7 +114,7 @@ def test_numbers_of_all_sizes_in_one_row(kernels, m, n, k, group, x_dtype):
     packed = kernels.pack_codes(codes, scales, group)
     values = values_of(codes, scales, group)
     out = torch.empty(m, n, device=DEV)
-    for small in (1.0, 2.0 ** -8, 2.0 ** -20, 2.0 ** -40, 2.0 ** -100):
+    for small in (1.0, 2.0 ** -8, 2.0 ** -20, 2.0 ** -40, 2.0 ** -119):
         for large in (2.0 ** 9, 2.0 ** 20, 2.0 ** 50, 2.0 ** 126):
             rows = x * small
             rows[:, at] = large
@@ -165,7 +166,8 @@ def rows_beyond_32_bits(g, m, n, k, group, x_dtype):
 
 @pytest.mark.parametrize("x_dtype", [BF16, F32])
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("m,n,k", [(1, 40, 64), (3, 70, 300), (7, 2048, 1024), (16, 33, 2048), (12, 64, 30000)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 64), (3, 70, 300), (7, 2048, 1024), (16, 33, 2048), (12, 64, 30000), (17, 40, 128), (20, 2048, 1024),
+                                   (90, 130, 2048), (300, 200, 72), (500, 4128, 512)])
 def test_sums_whose_way_passes_32_bits(kernels, m, n, k, group, x_dtype):
     g = gen(60 + m)
     x, codes, scales = rows_beyond_32_bits(g, m, n, k, group, x_dtype)
