@@ -53,3 +53,35 @@ def test_the_recurrences_ask_for_their_shared_memory_whatever_its_size():
 def test_rules_ask_the_device_for_its_sms(name):
     with open(os.path.join(CSRC, name)) as f:
         assert not re.findall(r"constexpr[^;]*\b148\b", re.sub(r"//[^\n]*", "", f.read()))
+
+
+def short_circuits(text):
+    """Lines where a warp-wide instruction stands behind && or || (or ?): lanes that decide early never come to it, and the others wait
+    for them."""
+    text = re.sub(r"//[^\n]*", "", text)
+    found = []
+    for m in re.finditer(r"\b__(?:shfl|any|all|ballot|reduce)\w*_sync\(|\b__syncthreads_\w+\(", text):
+        before = re.split(r"[;{}]", text[:m.start()])[-1]
+        depth, at = 0, len(before) - 1               # back to the start of this operand's expression, at its own depth of brackets
+        while at >= 0:
+            if before[at] == ")":
+                depth += 1
+            elif before[at] == "(":
+                depth = max(0, depth - 1)
+            elif depth == 0 and (before[at] == "?" or before[at - 1:at + 1] in ("&&", "||")):
+                found.append(text[:m.start()].count("\n") + 1)
+                break
+            at -= 1
+    return found
+
+
+def test_the_check_sees_a_shuffle_that_some_lanes_skip():
+    assert short_circuits("x = a || (__shfl_xor_sync(m, a, 8) && b);") == [1]
+    assert short_circuits("x = a ? __any_sync(m, b) : c;") == [1]
+    assert short_circuits("x = __shfl_xor_sync(m, a, 8);\ny = a || x;\nif (__any_sync(m, a && b) && c)\n  f(__ballot_sync(m, (a || b)));") == []
+
+
+@pytest.mark.parametrize("name", ["packed_weights.cu", "packed_tcgen05.cu", "packed.cuh"])
+def test_no_lane_skips_a_warps_instruction(name):
+    with open(os.path.join(CSRC, name)) as f:
+        assert short_circuits(f.read()) == []
