@@ -73,8 +73,8 @@ class GatedMLP(FeedForward):
                                            tensors[self.names["up_bias"]].to(gate.dtype)]).contiguous()
             self.bias_down = tensors[self.names["down_bias"]].float().contiguous()
         if self.runtime.weight_group is not None and self.fused_gate:
-            self.gate_up_interleaved = self.runtime.kernels.pack_gate_up(gate, up, self.runtime.weight_group)
-            self.down = self.runtime.pack(tensors[self.names["down_proj"]])
+            self.gate_up_interleaved = self.runtime.kernels.pack_gate_up(gate.contiguous(), up.contiguous(), self.runtime.weight_group)
+            self.down = self.runtime.pack(tensors[self.names["down_proj"]].contiguous())
             return
         interleave = getattr(self.runtime.kernels, "interleave_gate_up", None) if self.fused_gate else None
         self.gate_up_interleaved = interleave(gate, up) if interleave is not None else None

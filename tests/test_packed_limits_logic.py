@@ -6,10 +6,12 @@ import pytest
 import torch
 
 import chibillm_b200.csrc
+from chibillm_b200.config import GatedMLPSpec
 from chibillm_b200.engine.runner import make_runtime
 from chibillm_b200.kernels.ops import CudaKernels, KernelError
 from chibillm_b200.kernels import ops
 from chibillm_b200.kernels.packed import PackedWeights, few_rows_plan, many_rows_cut
+from chibillm_b200.parts import make_feed_forward
 from packed_models import PackedReferenceKernels
 
 
@@ -148,3 +150,32 @@ def test_a_query_that_failed_is_asked_again(monkeypatch):
             ask()
         Library.answers[which] = 148
         assert ask().clusters >= 1
+
+
+@pytest.mark.parametrize("activation,biases", [("silu", False), ("gelu_tanh", False), ("gelu_tanh", True)])
+def test_feed_forwards_take_matrices_in_another_order(activation, biases):
+    """Tensors whose rows are not contiguous are put in order before they are packed, as the other layouts do."""
+    class Strict(PackedReferenceKernels):
+        def pack_weights(self, w, group=64):
+            assert w.is_contiguous()
+            return super().pack_weights(w, group)
+
+        def pack_gate_up(self, gate, up, group=64):
+            assert gate.is_contiguous() and up.is_contiguous()
+            return super().pack_gate_up(gate, up, group)
+
+    g = torch.Generator().manual_seed(3)
+    names = {n: n for n in ("gate_proj", "up_proj", "down_proj", "gate_bias", "up_bias", "down_bias")}
+    tensors = {"gate_proj": torch.randn(96, 64, generator=g), "up_proj": torch.randn(96, 64, generator=g),
+               "down_proj": torch.randn(64, 96, generator=g), "gate_bias": torch.randn(96, generator=g),
+               "up_bias": torch.randn(96, generator=g), "down_bias": torch.randn(64, generator=g)}
+    spec = GatedMLPSpec("gated_mlp", hidden_size=64, intermediate_size=96, activation=activation, biases=biases)
+    bound = []
+    for order in (lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t):
+        runtime = make_runtime("float32", "cpu", kernels=Strict(), weight_group=32)
+        part = make_feed_forward(spec, names, runtime)
+        part.bind({n: order(t) for n, t in tensors.items()})
+        bound.append(part)
+    for name in ("gate_up", "gate_up_interleaved", "down"):
+        one, other = (getattr(p, name) for p in bound)
+        assert (one is None) == (other is None) and (one is None or torch.equal(one.values, other.values)), name
