@@ -51,6 +51,7 @@ the rows of every q and k head (and their biases and norm weights) put in anothe
 """
 from __future__ import annotations
 
+from collections import ChainMap
 from typing import Dict, List
 
 import torch
@@ -190,7 +191,7 @@ class PagedAttention(Mixer):
         order = self.position.feature_order()
         if order is not None:
             # the features of q and k in the order in which the kernels' rotation pairs them
-            tensors = dict(tensors)
+            tensors = ChainMap({}, tensors)
             d = self.spec.head_dim
             for r in ("q_proj", "k_proj", "q_bias", "k_bias", "q_norm", "k_norm"):
                 t = tensors.get(self.names.get(r))

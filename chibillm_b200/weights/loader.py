@@ -13,7 +13,9 @@ int32.
 """
 from __future__ import annotations
 
-from typing import Dict, List
+from collections.abc import Mapping
+from typing import Callable, Iterable, Iterator, List
+from weakref import WeakValueDictionary
 
 import torch
 
@@ -79,7 +81,37 @@ def device_dtype(stored: torch.dtype, kind: str, runtime_dtype: torch.dtype) -> 
     return torch.bfloat16
 
 
-def load_weights(model, model_dir: str, runtime: Runtime) -> Dict[str, torch.Tensor]:
+class DeviceTensors(Mapping):
+    """A model's tensors by name, each put on the device when a part asks for it and kept by whoever holds it: one that a part
+    has stacked with others, or packed, does not stay beside what was made of it.  Held by several, it is one tensor."""
+
+    def __init__(self, names: Iterable[str], make: Callable[[str], torch.Tensor]):
+        self._names, self._make = dict.fromkeys(names), make
+        self._held = WeakValueDictionary()
+
+    def __getitem__(self, name: str) -> torch.Tensor:
+        if name not in self._names:
+            raise KeyError(name)
+        t = self._held.get(name)
+        if t is None:
+            t = self._held[name] = self._make(name)
+        return t
+
+    def __contains__(self, name) -> bool:
+        return name in self._names
+
+    def __iter__(self) -> Iterator[str]:
+        return iter(self._names)
+
+    def __len__(self) -> int:
+        return len(self._names)
+
+
+def put_on_device(stored: torch.Tensor, kind: str, runtime: Runtime) -> torch.Tensor:
+    return stored.to(device=runtime.device, dtype=device_dtype(stored.dtype, kind, runtime.dtype), copy=True)
+
+
+def load_weights(model, model_dir: str, runtime: Runtime) -> DeviceTensors:
     """Check, read and hand the tensors to the model's parts."""
     try:
         checkpoint = Checkpoint.open_model(model_dir)
@@ -87,10 +119,7 @@ def load_weights(model, model_dir: str, runtime: Runtime) -> Dict[str, torch.Ten
         raise WeightError(str(e)) from None
     expected = model.expected_tensors(checkpoint.names())
     check_checkpoint(expected, checkpoint)
-    tensors: Dict[str, torch.Tensor] = {}
-    for spec in expected:
-        stored = checkpoint.read(spec.name)
-        target = device_dtype(stored.dtype, spec.kind, runtime.dtype)
-        tensors[spec.name] = stored.to(device=runtime.device, dtype=target, copy=True)
+    kinds = {spec.name: spec.kind for spec in expected}
+    tensors = DeviceTensors(kinds, lambda name: put_on_device(checkpoint.read(name), kinds[name], runtime))
     model.bind(tensors)
     return tensors

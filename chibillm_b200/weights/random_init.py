@@ -22,6 +22,7 @@ from typing import Iterator, Tuple
 import torch
 
 from ..parts.base import Runtime, TensorSpec
+from .loader import DeviceTensors
 from .safetensors_io import write_safetensors
 
 MATRIX_STD = 0.02
@@ -123,12 +124,14 @@ def write_random_model(config_object: dict, out_dir: str, seed: int,
     return out_dir
 
 
+def stored_tensor(spec: TensorSpec, seed: int, runtime: Runtime, stored: torch.dtype) -> torch.Tensor:
+    t = random_tensor(spec, seed, stored, runtime.device)
+    return t if t.dtype in (runtime.dtype, torch.int32) else t.to(runtime.dtype)
+
+
 def bind_random_weights(model, seed: int, runtime: Runtime, stored: torch.dtype = torch.bfloat16) -> None:
     """Fill a model with random weights made on its device (no file): the values
     that ``write_random_model`` would store as ``stored`` with the same seed,
     widened to the run's type as the loader widens a checkpoint's."""
-    tensors = {}
-    for spec in model.expected_tensors(None):
-        t = random_tensor(spec, seed, stored, runtime.device)
-        tensors[spec.name] = t if t.dtype in (runtime.dtype, torch.int32) else t.to(runtime.dtype)
-    model.bind(tensors)
+    specs = {spec.name: spec for spec in model.expected_tensors(None)}
+    model.bind(DeviceTensors(specs, lambda name: stored_tensor(specs[name], seed, runtime, stored)))

@@ -1,18 +1,24 @@
 """Matrices in 4 bits without a GPU: what must be refused or looked at before a kernel runs."""
+import math
 import os
 import re
+import weakref
 
 import pytest
 import torch
 
 import chibillm_b200.csrc
+import helpers
+import tiny_configs
 from chibillm_b200.config import GatedMLPSpec
-from chibillm_b200.engine.runner import make_runtime
+from chibillm_b200.engine.runner import ModelRunner, make_runtime
 from chibillm_b200.kernels.ops import CudaKernels, KernelError
 from chibillm_b200.kernels import ops
 from chibillm_b200.kernels.packed import PackedWeights, few_rows_plan, many_rows_cut
 from chibillm_b200.parts import make_feed_forward
+from chibillm_b200.weights import loader, random_init
 from packed_models import PackedReferenceKernels
+from reference_ops import ReferenceKernels
 
 
 def smem_kb(wide, group, columns):
@@ -179,3 +185,53 @@ def test_feed_forwards_take_matrices_in_another_order(activation, biases):
     for name in ("gate_up", "gate_up_interleaved", "down"):
         one, other = (getattr(p, name) for p in bound)
         assert (one is None) == (other is None) and (one is None or torch.equal(one.values, other.values)), name
+
+
+def live_bytes_while(monkeypatch, load):
+    """The most bytes of source tensors on the device at any time while ``load`` runs (counted where a part asks for one)."""
+    live, most = {}, [0]
+
+    def watched(make):
+        def made(*args, **kw):
+            t = make(*args, **kw)
+            key = id(t)
+            live[key] = t.numel() * t.element_size()
+            weakref.finalize(t, live.pop, key, None)
+            most[0] = max(most[0], sum(live.values()))
+            return t
+        return made
+
+    monkeypatch.setattr(loader, "put_on_device", watched(loader.put_on_device))
+    monkeypatch.setattr(random_init, "stored_tensor", watched(random_init.stored_tensor))
+    load()
+    return most[0]
+
+
+@pytest.mark.parametrize("name", ["A", "B"])
+@pytest.mark.parametrize("from_folder", [True, False])
+def test_a_model_is_never_whole_on_the_device_beside_its_packed_matrices(tmp_path, monkeypatch, name, from_folder):
+    """Packing while a model is loaded: a matrix goes when it has been packed, so what fits in 4 bits can be loaded."""
+    config = dict(tiny_configs.get(name), num_hidden_layers=12)
+    folder = helpers.make_model_dir(tmp_path, name, seed=3, num_hidden_layers=12)
+    kernels = PackedReferenceKernels()
+    common = dict(dtype="float32", device="cpu", page_size=8, pool_tokens=192, kernels=kernels, weight_group=32)
+    runners = []
+    most = live_bytes_while(monkeypatch, lambda: runners.append(
+        ModelRunner.from_folder(folder, **common) if from_folder else ModelRunner.from_random(config, seed=3, **common)))
+    spec = runners[0].model.spec
+    sizes = {t.name: math.prod(t.shape) * 4 for t in runners[0].model.expected_tensors(None)}
+    kept = sum(n for name, n in sizes.items() if "norm" in name) + sizes[spec.embedding_name] + sizes.get(spec.output_name, 0)
+    layer = sum(n for name, n in sizes.items() if ".layers.0." in name)
+    assert most <= kept + layer < sum(sizes.values()) / 3
+
+
+def test_loaded_tensors_are_one_while_somebody_holds_them(tmp_path):
+    folder = helpers.make_model_dir(tmp_path, "A", seed=3)
+    runner = ModelRunner.from_folder(folder, dtype="float32", device="cpu", page_size=8, pool_tokens=192, kernels=ReferenceKernels())
+    tensors = loader.load_weights(runner.model, folder, runner.runtime)
+    names = list(tensors)
+    held = tensors[names[0]]
+    assert tensors[names[0]] is held and names[0] in tensors and "no such" not in tensors and None not in tensors
+    assert tensors.get(None) is None and len(tensors) == len(names) == len(set(names))
+    with pytest.raises(KeyError):
+        tensors["no such"]
