@@ -281,14 +281,6 @@ __device__ __forceinline__ void tmem_load_32x16(uint32_t taddr, uint32_t (&r)[16
                  : "memory");
 }
 
-__device__ __forceinline__ void tmem_load_32x8(uint32_t taddr, uint32_t (&r)[8])
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(taddr)
-                 : "memory");
-}
-
 // The mirror of tmem_load_32x32: thread i writes columns [col, col + 32) of its lane.
 __device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t (&r)[32])
 {
