@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) packed_many_rows_kernel(const _
                     break;
                 }
                 const uint8_t* rec = codes + s * T::CODE_BYTES + quarter * RECORD;
-                uint32_t w[4][4];                // [piece][word]
+                __align__(16) uint32_t w[4][4];  // [piece][word]
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     *reinterpret_cast<uint4*>(w[c]) = *reinterpret_cast<const uint4*>(rec + packed_word_at(lane, c));

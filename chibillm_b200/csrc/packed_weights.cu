@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(128, 8) pack_kernel(PackSource p, int row_bloc
         // (a row beyond the matrix is read as one without columns)
         const T* src = base + (row < p.rows ? (long long)row * stride : 0);
         const int cols = row < p.rows ? p.cols : 0;
-        T raw[4][8];
+        __align__(16) T raw[4][8];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             read_eight(src, col + c * 8, cols, raw[c]);
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
             if (row >= rows || col >= cols)
                 continue;
             T* dst = out + (long long)(row + packed_side(pair, r) * rows) * stride + col;
-            T v[EACH];
+            __align__(16) T v[EACH];
 #pragma unroll
             for (int j = 0; j < EACH; ++j) {
                 const int e = (first & 7) + j;
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
                 const int here = min(todo, p.run);
                 todo -= here;
                 for (int j = 0; j < here; ++j, rec += RECORD, rec_scales += RECORD, x_at += 4 * x_block) {
-                    uint32_t w[4][4];                        // rows r, r + 8, r + 16, r + 24
+                    __align__(16) uint32_t w[4][4];          // rows r, r + 8, r + 16, r + 24
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(rec + i * 512);

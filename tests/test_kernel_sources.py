@@ -85,3 +85,12 @@ def test_the_check_sees_a_shuffle_that_some_lanes_skip():
 def test_no_lane_skips_a_warps_instruction(name):
     with open(os.path.join(CSRC, name)) as f:
         assert short_circuits(f.read()) == []
+
+
+@pytest.mark.parametrize("name", ["packed_weights.cu", "packed_tcgen05.cu", "packed.cuh"])
+def test_arrays_that_are_read_as_16_bytes_start_on_16(name):
+    with open(os.path.join(CSRC, name)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    cast = set(re.findall(r"reinterpret_cast<(?:const )?uint4\*>\((\w+)", text))
+    for m in re.finditer(r"^[ \t]*((?:__align__\(16\) )?)(?:T|float|uint32_t) (\w+)(?:\[\w+\])+[^;()]*;", text, re.M):
+        assert m.group(2) not in cast or m.group(1), m.group(0)
