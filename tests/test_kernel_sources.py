@@ -91,6 +91,7 @@ def test_no_lane_skips_a_warps_instruction(name):
 def test_arrays_that_are_read_as_16_bytes_start_on_16(name):
     with open(os.path.join(CSRC, name)) as f:
         text = re.sub(r"//[^\n]*", "", f.read())
-    cast = set(re.findall(r"reinterpret_cast<(?:const )?uint4\*>\((\w+)", text))
-    for m in re.finditer(r"^[ \t]*((?:__align__\(16\) )?)(?:T|float|uint32_t) (\w+)(?:\[\w+\])+[^;()]*;", text, re.M):
-        assert m.group(2) not in cast or m.group(1), m.group(0)
+    for cast in re.finditer(r"reinterpret_cast<(?:const )?uint4\*>\((\w+)", text):
+        # (the nearest declaration of that name above; a reference's array is its caller's)
+        declared = re.findall(r"((?:__align__\(16\) )?)\b(?:T|float|uint32_t) (\(&)?" + cast.group(1) + r"\)?\[", text[:cast.start()])
+        assert not declared or declared[-1][0] or declared[-1][1], text[cast.start():].split("\n")[0]
