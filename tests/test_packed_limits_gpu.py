@@ -196,3 +196,58 @@ def test_sums_whose_way_passes_32_bits(kernels, m, n, k, group, x_dtype):
     # (expf and the division are good to 2 half steps each, the product to one; gate and up are exact)
     assert ((gated.double() - want).abs() <= want.abs() * 8 * 2.0 ** -24 + 2.0 ** -149)[fits].all()
     kernels.check_error_word()
+
+
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("m,n,k", [(1, 151936, 256), (1, 128, 32768), (2, 64, 65536), (16, 64, 20000), (9, 40, 65531), (40, 64, 20000),
+                                   (300, 200, 4104), (1, 6144, 4096), (24, 6144, 4096), (70, 129, 1)])
+def test_no_element_of_a_long_row_hides(kernels, m, n, k, group, x_dtype):
+    """Whole numbers whose sums are exact (65,536 * 8 * 4 * 2 < 2^24 steps): an element that is dropped, taken twice or swapped with
+    another shows, wherever it is."""
+    g = gen(70 + m)
+    codes = torch.randint(-8, 8, (n, k), generator=g, device=DEV, dtype=torch.int8)
+    scales = (2.0 ** torch.randint(-1, 1, (n, -(-k // group)), generator=g, device=DEV)).to(BF16)
+    x = torch.randint(-4, 5, (m, k), generator=g, device=DEV).to(x_dtype)
+    out = torch.empty(m, n, device=DEV)
+    kernels.linear(x, kernels.pack_codes(codes, scales, group), out)
+    for at in range(0, n, 8192):
+        assert torch.equal(out[:, at:at + 8192].double(), x.double() @ values_of(codes[at:at + 8192], scales[at:at + 8192], group).t())
+    kernels.check_error_word()
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 70, 512), (5, 2730, 1024), (12, 33, 2048), (16, 64, 4096), (17, 65, 512), (60, 300, 1024), (200, 1000, 136)])
+def test_no_element_of_a_pair_hides(kernels, m, n, k, x_dtype, kind):
+    """Gates from 32 on come out of both activations as they are, in 32 bits (exp(-32) is below half a step of 1): exact again.  The
+    largest, 4,096 * 7 * 3 * 2, times the largest up, 7 * 3, is below 2^24 halves."""
+    g = gen(71 + m)
+    codes = torch.randint(0, 8, (n, k), generator=g, device=DEV, dtype=torch.int8)
+    few = torch.zeros(n, k, dtype=torch.int8, device=DEV)
+    few[torch.arange(n, device=DEV), torch.randint(0, k, (n,), generator=g, device=DEV)] = 7
+    scales = torch.ones(n, -(-k // 64), dtype=BF16, device=DEV)
+    x = torch.randint(1, 4, (m, k), generator=g, device=DEV).to(x_dtype)
+    gate, up = x.double() @ codes.double().t(), x.double() @ few.double().t()
+    assert gate.min() > 32 and (gate * up).max() < 2.0 ** 24
+    out = torch.empty(m, n, device=DEV)
+    kernels.linear_swiglu(x, kernels.pack_codes(codes, scales, 64, few, scales), out, kind=kind)
+    assert torch.equal(out.double(), gate * up)
+    kernels.check_error_word()
+
+
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+@pytest.mark.parametrize("m", [1, 9, 16, 17, 60, 400])
+def test_a_residual_beside_bfloat16_outputs(kernels, m, x_dtype):
+    """The residual is added to the 32-bit sums, before they are rounded."""
+    g = gen(72 + m)
+    w = matrix(g, 300, 512, BF16)
+    packed, values = kernels.pack_weights(w, 64), packed_values(w, 64)
+    x = torch.randn(m, 512, generator=g, device=DEV).to(x_dtype)
+    add = torch.randn(m, 640, generator=g, device=DEV)[:, 5:305]
+    out = torch.empty(m, 300, dtype=BF16, device=DEV)
+    kernels.linear(x, packed, out, residual=add)
+    want = x.double() @ values.t()
+    bound = off_by(x, values, 64, F32, want) + want.abs() * 2.0 ** -24
+    want = want + add.double()
+    close(out, want, bound * (1 + 2.0 ** -8) + want.abs() * 2.0 ** -8)
