@@ -280,8 +280,8 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // off by 2^-23 of themselves, or by 2^-25, half of float16's last step, which is 2^-39 of the row's largest at most and 2^-16 of
 // numbers from 2^-9 on.  What is smaller (bfloat16: 2^-14, 32-bit: 2^-9, as multiplied) and lost bits is added to the warps' sums in
 // 32 bits after the stream, so nothing vanishes beside a large number whose weights are zeros (add_what_was_lost; a row of 4,096 normal
-// numbers has one with a chance of 1e-5, a 32-bit one of 1e-3; one such number makes the product with 4,096 x 4,096 take 6.8 us
-// instead of 4.8, a row of nothing else 30).
+// numbers has one with a chance of 1e-5, a 32-bit one of 1e-3; one such number makes the product with 4,096 x 4,096 take 7.5 us
+// instead of 4.8, a row of nothing else 36).
 //
 // How the work is shared out (CudaKernels.packed_plan chooses): `splits` CTAs of a cluster share the columns, `along_k`
 // warps of a CTA share the CTA's columns of one block of 32 rows, the CTA's warps / along_k blocks of rows are a unit, and clusters
@@ -447,7 +447,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     const int most = (p.chunks + splits - 1) >> p.split_shift;
     const int unit_shift = (p.warps == 16 ? 4 : 3) - p.along_shift, blocks_per_unit = 1 << unit_shift;
 
-    // shared memory: rings | x | sums | the rows' largest numbers, a bit for each that lost bits | barriers
+    // shared memory: rings | x | sums | the rows' largest numbers, a bit for each that lost bits, a bit for each with a factor of its
+    // own | barriers
     const uint32_t x_plane = (uint32_t)most * 4 * p.tokens * 64;
     const int stage = (p.run * RECORD + 127) / 128 * 128;        // (a tile copy's place starts on 128 bytes)
     uint8_t* ring = smem + warp * p.depth * stage;
@@ -495,25 +496,24 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     const int token_turn = warp / tokens, token = warp - token_turn * tokens;
     const int first_piece = token_turn < token_warps ? token_turn * 32 + lane : token_pieces, step = token_warps * 32;
     const T* x_row = static_cast<const T*>(p.x) + (token0 + token) * p.x_stride;
-    uint8_t* x_to = xs + token * 64;
-    auto put = [&](int i, const T (&raw)[8], float up_by) {
+    auto put = [&](int of, int i, const T (&raw)[8], float up_by) {
         float pairs[4][2];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             pairs[j / 2][j % 2] = to_f32(raw[j]) * up_by;
-        uint8_t* dst = x_to + (i >> 2) * p.tokens * 64 + (i & 3) * 16;
+        uint8_t* dst = xs + of * 64 + (i >> 2) * p.tokens * 64 + (i & 3) * 16;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
             *reinterpret_cast<uint4*>(dst + part * x_plane)
                 = make_uint4(take_half_pair(pairs[0]), take_half_pair(pairs[1]), take_half_pair(pairs[2]), take_half_pair(pairs[3]));
     };
-    // 32-bit rows are looked at first.  bfloat16 rows are multiplied by 2^6 at once, and only if a CTA has a number that this does not suit
-    // (two at a time, their bits as whole numbers; less 1, so that a zero is the largest of all) are its rows looked at and what has
-    // to be is done once more.
+    // 32-bit rows are looked at first.  bfloat16 rows are multiplied by 2^6 at once, and only those with a number that this does not suit
+    // (two at a time, their bits as whole numbers; less 1, so that a zero is the largest of all) are looked at, and done once more by
+    // the whole CTA: 8 rows through a gated pair of 2 x 12,288 x 4,096 16.7 us, with one such row 17.8, all of them such 21.9.
     constexpr float AT_FIRST = float(1 << ROW_EXPONENT);
     uint32_t most_two = 0, least_two = 0xffffffffu;
     auto put_at_first = [&](int i, const T (&raw)[8]) {
-        put(i, raw, AT_FIRST);
+        put(token, i, raw, AT_FIRST);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t two = reinterpret_cast<const uint32_t*>(raw)[j] & 0x7fff7fffu;
@@ -526,6 +526,27 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             most_of = fmaxf(most_of, fabsf(to_f32(raw[j])));
+    };
+    auto look_at_finite = [&](const T (&raw)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            most_of = fabsf(to_f32(raw[j])) < INFINITY ? fmaxf(most_of, fabsf(to_f32(raw[j]))) : most_of;
+    };
+    // pieces of a row whose largest number is known, with its factor, and whether they have numbers that lose bits
+    auto put_and_note = [&](int of, const T* row, int piece0, int pieces) {
+        const int e = row_exponent(largest[of]);
+        uint32_t smallest = 0xffffffffu;         // but zero, its bits less 1
+#pragma unroll 1
+        for (int i = piece0; i < token_pieces; i += pieces) {
+            __align__(16) T raw[8];
+            read_eight(row, (c0 * 16 + i) * 8, p.k, raw);
+            put(of, i, raw, power_of_two(e));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                smallest = __viaddmin_u32(__float_as_uint(to_f32(raw[j])) & 0x7fffffffu, 0xffffffffu, smallest);
+        }
+        if (smallest < __float_as_uint(least_kept<X32>() * power_of_two(-e)) - 1)
+            atomicOr(&largest[16], 1u << of);
     };
     if (((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)p.x_stride * sizeof(T)) & 15) == 0 && (p.k & 7) == 0) {
         // whole pieces on 16 bytes
@@ -566,18 +587,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
                 put_at_first(i, raw);
         }
     }
-    bool looked_at = true;
-    if constexpr (!X32) {
-        looked_at = __syncthreads_or(max(most_two >> 16, most_two & 0xffffu) >= ROW_MOST << 7 || min(least_two >> 16, least_two & 0xffffu) < (ROW_LEAST << 7) - 1);
-        if (__builtin_expect(looked_at, false))
-#pragma unroll 1
-            for (int i = first_piece; i < token_pieces; i += step) {
-                __align__(16) T raw[8];
-                read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
-                look(raw);
-            }
-    }
-    if (__builtin_expect(looked_at, X32)) {
+    uint32_t own_factor = 0;                     // the rows with a factor of their own
+    if constexpr (X32) {
         uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
         if (warps_most == 0x7f800000u) {         // (an infinity: the largest of the others; fmaxf passes NaN over)
             most_of = 0.f;
@@ -585,29 +596,43 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
             for (int i = first_piece; i < token_pieces; i += step) {
                 __align__(16) T raw[8];
                 read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    most_of = fabsf(to_f32(raw[j])) < INFINITY ? fmaxf(most_of, fabsf(to_f32(raw[j]))) : most_of;
+                look_at_finite(raw);
             }
             warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
         }
         if (lane == 0)
             atomicMax(&largest[token], warps_most);
         __syncthreads();
-        const int e = row_exponent(largest[token]);
-        uint32_t smallest = 0xffffffffu;         // but zero, its bits less 1
-#pragma unroll 1
-        for (int i = first_piece; i < token_pieces; i += step) {
-            __align__(16) T raw[8];
-            read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
-            put(i, raw, power_of_two(e));
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                smallest = __viaddmin_u32(__float_as_uint(to_f32(raw[j])) & 0x7fffffffu, 0xffffffffu, smallest);
-        }
-        if (smallest < __float_as_uint(least_kept<X32>() * power_of_two(-e)) - 1)
-            atomicOr(&largest[16], 1u << token);
+        put_and_note(token, x_row, first_piece, step);
         __syncthreads();
+        own_factor = 0xffffffffu;
+    } else {
+        const bool odd = max(most_two >> 16, most_two & 0xffffu) >= ROW_MOST << 7 || min(least_two >> 16, least_two & 0xffffu) < (ROW_LEAST << 7) - 1;
+        if (odd)
+            atomicOr(&largest[17], 1u << token);
+        if (__builtin_expect(__syncthreads_or(odd), false)) {
+            own_factor = largest[17];
+            // (the warps share them as they shared all)
+            const int rows = __popc(own_factor), turn = warp / rows, each = p.warps / rows;
+            uint32_t from = own_factor;
+            for (int skip = warp - turn * rows; skip > 0; --skip)
+                from &= from - 1;
+            const int of = __ffs(from) - 1;
+            const int piece0 = turn < each ? turn * 32 + lane : token_pieces;
+            const T* row = x_row + (of - token) * p.x_stride;
+#pragma unroll 1
+            for (int i = piece0; i < token_pieces; i += each * 32) {
+                __align__(16) T raw[8];
+                read_eight(row, (c0 * 16 + i) * 8, p.k, raw);
+                look_at_finite(raw);
+            }
+            const uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
+            if (lane == 0)
+                atomicMax(&largest[of], warps_most);
+            __syncthreads();
+            put_and_note(of, row, piece0, each * 32);
+            __syncthreads();
+        }
     }
 
     // ---- the stream
@@ -623,13 +648,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
             down[t][j] = 1.f / AT_FIRST;
     }
     uint32_t lossy = 0;                          // the rows with numbers that lost bits
-    if (__builtin_expect(looked_at, X32)) {
+    if (__builtin_expect(own_factor != 0, X32)) {
         lossy = largest[16];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                down[t][j] = power_of_two(-row_exponent(largest[min(t * 8 + 2 * c + j, tokens - 1)]));
+            for (int j = 0; j < 2; ++j) {
+                const int of = min(t * 8 + 2 * c + j, tokens - 1);
+                down[t][j] = own_factor >> of & 1 ? power_of_two(-row_exponent(largest[of])) : down[t][j];
+            }
     }
     const uint32_t x_block = (uint32_t)p.tokens * 64;
     bool dead = false;                           // a wait ran out: nothing more is asked for
