@@ -91,8 +91,11 @@ inline bool packed_map(const void* data, int group, int row_blocks, int col_bloc
               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The whole numbers of a word as float16, columns 2 j and 2 j + 1 in pair j (exact: 1,024 + code and 1,024 + 16 code have
-// the code in float16's ten bits of mantissa, and what is taken off leaves a small whole number).
+// The whole numbers of a word as float16, columns 2 j and 2 j + 1 in pair j, times 2^-14 (exact: 1,024 + code and 1,024 + 16 code have
+// the code in float16's ten bits of mantissa, a way that open 4-bit kernels share; what is taken off leaves a small whole number).
+// x is held at 2^15 at most, so a group's sum is below 2^11 and its product with a scale finite for scales below 2^117, weights of
+// 10^36.  PACKED_HALF_EXPONENT undoes it.
+constexpr int PACKED_HALF_EXPONENT = 14;
 __device__ __forceinline__ void packed_half_pairs(uint32_t word, uint32_t (&pair)[4])
 {
     const uint32_t next = word >> 8;
@@ -100,10 +103,10 @@ __device__ __forceinline__ void packed_half_pairs(uint32_t word, uint32_t (&pair
     asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(pair[1]) : "r"(word));
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(pair[2]) : "r"(next));
     asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(pair[3]) : "r"(next));
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(pair[0]) : "r"(0x64086408u));                       // - 1,032
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[1]) : "r"(0x2c002c00u), "r"(0xd480d480u)); // / 16 - 72
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(pair[2]) : "r"(0x64086408u));
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[3]) : "r"(0x2c002c00u), "r"(0xd480d480u));
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[0]) : "r"(0x04000400u), "r"(0xac08ac08u)); // * 2^-14 - 1,032 * 2^-14
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[1]) : "r"(0x00400040u), "r"(0x9c809c80u)); // * 2^-18 - 1,152 * 2^-18
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[2]) : "r"(0x04000400u), "r"(0xac08ac08u));
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[3]) : "r"(0x00400040u), "r"(0x9c809c80u));
 }
 
 // The same as bfloat16, times 2^-10 (2^-3 + 2^-10 code has its code in the lowest of bfloat16's seven bits of mantissa).  A group's
@@ -126,61 +129,6 @@ template <bool ROUNDED> __device__ __forceinline__ float packed_activate(float z
 {
     const float y = act == 2 ? z : 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
     return ROUNDED ? __fdividef(z, 1.f + __expf(-y)) : z / (1.f + expf(-y));
-}
-
-// 8 neighbouring numbers of a row from column `col` on, zeros beyond its k columns.
-template <typename T> __device__ __forceinline__ void read_eight(const T* row, int col, int k, T (&v)[8])
-{
-    const T* src = row + col;
-    if (col + 8 <= k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-            reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = col + i < k ? src[i] : from_f32<T>(0.f);
-    }
-}
-
-// Products of rows of the matrix with rows of x, by a warp each and in 64 bits: for sums that came out as no number although every
-// number of x is one (a group's sum, or its product with a scale, can pass 2^128 where the whole does not: weights from 10^32 on,
-// x from 10^35 on).  Terms are exact (4, 8 and 24 bits).  The whole warp calls; a lane that asks has the block of rows, the row in
-// its records and the row of x, and gets the sum instead of v.  Slow, 6 us for 4,096 columns (less where a NaN ends it).
-template <typename T>
-__device__ __forceinline__ float packed_sums_in_64_bits(const uint8_t* data, int group, int chunks, int k, bool asks, int block, int r,
-                                                        const T* x, float v)
-{
-    const int lane = threadIdx.x & 31;
-#pragma unroll 1
-    for (uint32_t todo = __ballot_sync(0xffffffffu, asks); todo != 0; todo &= todo - 1) {
-        const int who = __ffs(todo) - 1;
-        const int row = __shfl_sync(0xffffffffu, r, who);
-        const uint8_t* rec = data + (long long)__shfl_sync(0xffffffffu, block, who) * chunks * packed_record_bytes(group);
-        const T* from = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(x), who));
-        double sum = 0.;
-#pragma unroll 1
-        for (int col = lane * 8; __any_sync(0xffffffffu, col < k); col += 256) {
-            if (col < k) {
-                __align__(16) T eight[8];
-                read_eight(from, col, k, eight);
-                const uint8_t* at = rec + (long long)(col / PACKED_COLS) * packed_record_bytes(group);
-                const uint32_t word = *reinterpret_cast<const uint32_t*>(at + packed_word_at(row, col % PACKED_COLS >> 3));
-                double part = 0.;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    part = fma((double)((int)((word >> (4 * (i / 2) + 16 * (i & 1))) & 15u) - 8), (double)to_f32(eight[i]), part);
-                sum = fma((double)to_f32(*reinterpret_cast<const __nv_bfloat16*>(at + packed_scale_at(row, col % PACKED_COLS / group))), part, sum);
-            }
-            if (__any_sync(0xffffffffu, sum != sum))
-                break;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        v = lane == who ? (float)sum : v;
-    }
-    return v;
 }
 
 } // namespace chibi

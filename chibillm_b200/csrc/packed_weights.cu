@@ -70,6 +70,21 @@ template <typename T> __device__ __forceinline__ uint32_t code_word(const T (&w)
     return word;
 }
 
+// 8 neighbouring numbers of a row from column `col` on, zeros beyond its k columns.
+template <typename T> __device__ __forceinline__ void read_eight(const T* row, int col, int k, T (&v)[8])
+{
+    const T* src = row + col;
+    if (col + 8 <= k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = col + i < k ? src[i] : from_f32<T>(0.f);
+    }
+}
+
 // Products fetch their matrix before the kernel ahead of them has ended.  So the kernels that write one, in 4 bits or as values read
 // back, let nothing start early (no pdl_trigger; and no mark in a timeline), and every thread's stores are performed, for tile copies
 // too, before it ends.
@@ -270,7 +285,8 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // (tile copies into a ring of its own, no barrier between warps), makes float16 fragments of the codes and multiplies
 // them with x by `mma.m16n8k16`: 16 rows of a record are the instruction's rows, 8 tokens its columns.  x lies in shared
 // memory as the fragments want it, 16 bytes to a lane for four instructions.  Each group's sums start at zero and are
-// multiplied by the scales in 32 bits.
+// multiplied by the scales in 32 bits.  (The codes are held times 2^-14, so that this does not pass 2^128 where a row of x has been
+// multiplied: 2^-100 times 64 sevens of scale 2^106 came out infinite.)
 //
 // x becomes float16 too (two nibbles of a word are float16 numbers without a shift, which bfloat16's seven bits of mantissa
 // do not allow; the conversion of the codes is most of the kernel's instructions).  A row's numbers, as far as the CTA's columns go, are
@@ -280,7 +296,7 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // off by 2^-23 of themselves, or by 2^-25, half of float16's last step, which is 2^-39 of the row's largest at most and 2^-16 of
 // numbers from 2^-9 on.  What is smaller (bfloat16: 2^-14, 32-bit: 2^-9, as multiplied) and lost bits is added to the warps' sums in
 // 32 bits after the stream, so nothing vanishes beside a large number whose weights are zeros (add_what_was_lost; a row of 4,096 normal
-// numbers has one with a chance of 1e-5, a 32-bit one of 1e-3; one such number makes the product with 4,096 x 4,096 take 7.5 us
+// numbers has one with a chance of 1e-5, a 32-bit one of 1e-3; one such number makes the product with 4,096 x 4,096 take 7.4 us
 // instead of 4.8, a row of nothing else 36).
 //
 // How the work is shared out (CudaKernels.packed_plan chooses): `splits` CTAs of a cluster share the columns, `along_k`
@@ -288,8 +304,8 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // take units in turn.  The sums of up to `batch` units stay in shared memory; then the cluster adds them up in one order
 // (each CTA its warps, then CTA by CTA), each CTA a share of the outputs, so the same plan gives the same bits.
 //
-// Measured (replayed in a graph, matrices out of L2): one row of 2,048 x 1,024 3.0 us, of 4,096 x 4,096 4.7, of 4,096 x 12,288 8.9, of a gated
-// pair of 2 x 12,288 x 4,096 13.0 (4.1 TB/s); four rows of 151,936 x 4,096 63.7 (5.2 TB/s), 284 instructions a record at 2.55 a
+// Measured (replayed in a graph, matrices out of L2): one row of 2,048 x 1,024 3.0 us, of 4,096 x 4,096 4.8, of 4,096 x 12,288 9.0, of a gated
+// pair of 2 x 12,288 x 4,096 13.3 (4.0 TB/s); four rows of 151,936 x 4,096 65.2 (5.1 TB/s), 284 instructions a record at 2.55 a
 // cycle and SM; 12 32-bit rows of a pair of 2 x 2,730 x 1,024 6.4.  Before and after the stream of one row go by 2.5 us: a kernel's start, x from
 // L2, a barrier, the warps' sums.
 constexpr int FEW_THREADS = 512;             // at most
@@ -341,6 +357,11 @@ __device__ __forceinline__ int row_exponent(uint32_t largest_bits)
 {
     return largest_bits == 0 ? 0 : min(14 + 127 - (int)(largest_bits >> 23), 126);
 }
+struct RowNotes {
+    uint32_t largest[16];          // their largest finite magnitudes, as bits (where a row's factor is its own)
+    int exponent[16];              // of their factors
+    uint32_t lossy, odd;           // a bit for each that lost bits; for each that the first factor does not suit
+};
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
 // Two numbers as float16, and what is left of them (nothing of an infinity or NaN).
@@ -368,14 +389,14 @@ template <bool X32> __device__ __forceinline__ float lost_of(float v, int e)
 // lane a row of the matrix.  A number that lost nothing costs its test alone, 32 columns at a time.
 template <bool X32, int NT>
 __device__ __noinline__ void add_what_was_lost(const FewRows& p, uint32_t rows, int token0, int block, int w0, int w1, int group,
-                                               const uint32_t* largest, float* sums)
+                                               const RowNotes& notes, float* sums)
 {
     using T = typename std::conditional<X32, float, __nv_bfloat16>::type;
     const int lane = threadIdx.x & 31;
     for (; rows != 0; rows &= rows - 1) {
         const int token = __ffs(rows) - 1;
         const T* x = static_cast<const T*>(p.x) + (token0 + token) * p.x_stride;
-        const int e = row_exponent(largest[token]);
+        const int e = notes.exponent[token];
         float sum = 0.f;
 #pragma unroll 1
         for (int chunk = w0; chunk < w1; ++chunk) {
@@ -412,16 +433,59 @@ __device__ __noinline__ void add_what_was_lost(const FewRows& p, uint32_t rows, 
     }
 }
 
-// (v, up) with the sums in 64 bits where they are no numbers (packed_sums_in_64_bits).
-template <bool X32>
-__device__ __noinline__ float2 sums_in_64_bits(const FewRows& p, int group, bool there, int block, int r, int m, float2 v)
+// 8 neighbouring numbers of a row as float16, for a lane of four instructions; 32-bit ones in two parts, `plane` bytes apart.
+template <typename T> __device__ __forceinline__ void put_piece(uint8_t* to, uint32_t plane, const T (&raw)[8], float up_by)
 {
-    using T = typename std::conditional<X32, float, __nv_bfloat16>::type;
-    const T* x = static_cast<const T*>(p.x) + m * p.x_stride;
-    v.x = packed_sums_in_64_bits(p.data, group, p.chunks, p.k, there && !isfinite(v.x), block, r, x, v.x);
-    if (p.pair)
-        v.y = packed_sums_in_64_bits(p.data, group, p.chunks, p.k, there && !isfinite(v.y), block, r + 8, x, v.y);
-    return v;
+    float pairs[4][2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        pairs[j / 2][j % 2] = to_f32(raw[j]) * up_by;
+#pragma unroll
+    for (int part = 0; part < (int)sizeof(T) / 2; ++part)
+        *reinterpret_cast<uint4*>(to + part * plane)
+            = make_uint4(take_half_pair(pairs[0]), take_half_pair(pairs[1]), take_half_pair(pairs[2]), take_half_pair(pairs[3]));
+}
+
+// bfloat16 rows that the first factor does not suit, once more, by all warps; `piece`s of a row's columns c0 * 128 ....  Begins
+// and ends with the CTA together.
+__device__ __noinline__ void put_rows_again(const FewRows& p, uint8_t* xs, RowNotes& notes, int token0, int c0, int pieces)
+{
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t odd = notes.odd;
+    const int rows = __popc(odd), turn = warp / rows, each = p.warps / rows;
+    uint32_t from = odd;
+    for (int skip = warp - turn * rows; skip > 0; --skip)
+        from &= from - 1;
+    const int of = __ffs(from) - 1, first = turn < each ? turn * 32 + lane : pieces;
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.x) + (token0 + of) * p.x_stride;
+    float most = 0.f, least = INFINITY;
+#pragma unroll 1
+    for (int i = first; i < pieces; i += each * 32) {
+        __align__(16) __nv_bfloat16 raw[8];
+        read_eight(row, (c0 * 16 + i) * 8, p.k, raw);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = fabsf(to_f32(raw[j]));
+            most = v < INFINITY ? fmaxf(most, v) : most;
+            least = v > 0.f ? fminf(least, v) : least;
+        }
+    }
+    const uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    if (lane == 0)
+        atomicMax(&notes.largest[of], warps_most);
+    __syncthreads();
+    const int e = row_exponent(notes.largest[of]);
+    if (least < least_kept<false>() * power_of_two(-e))
+        atomicOr(&notes.lossy, 1u << of);
+    if (lane == 0)
+        notes.exponent[of] = e;
+#pragma unroll 1
+    for (int i = first; i < pieces; i += each * 32) {
+        __align__(16) __nv_bfloat16 raw[8];
+        read_eight(row, (c0 * 16 + i) * 8, p.k, raw);
+        put_piece(xs + of * 64 + (i >> 2) * p.tokens * 64 + (i & 3) * 16, 0, raw, power_of_two(e));
+    }
+    __syncthreads();
 }
 
 template <int NT, bool X32, int GROUP_BLOCKS>
@@ -447,15 +511,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     const int most = (p.chunks + splits - 1) >> p.split_shift;
     const int unit_shift = (p.warps == 16 ? 4 : 3) - p.along_shift, blocks_per_unit = 1 << unit_shift;
 
-    // shared memory: rings | x | sums | the rows' largest numbers, a bit for each that lost bits, a bit for each with a factor of its
-    // own | barriers
+    // shared memory: rings | x | sums | notes about the rows of x (RowNotes) | barriers
     const uint32_t x_plane = (uint32_t)most * 4 * p.tokens * 64;
     const int stage = (p.run * RECORD + 127) / 128 * 128;        // (a tile copy's place starts on 128 bytes)
     uint8_t* ring = smem + warp * p.depth * stage;
     uint8_t* xs = smem + p.warps * p.depth * stage;
     float* sums = reinterpret_cast<float*>(xs + (size_t)PARTS * x_plane);
-    uint32_t* largest = reinterpret_cast<uint32_t*>(sums + p.batch * p.warps * SUMS);
-    uint64_t* full = reinterpret_cast<uint64_t*>(largest + 18) + warp * p.depth;
+    RowNotes& notes = *reinterpret_cast<RowNotes*>(sums + p.batch * p.warps * SUMS);
+    uint64_t* full = reinterpret_cast<uint64_t*>(&notes + 1) + warp * p.depth;
 
     // the warp's records: of its block of rows in every unit, columns w0 ... w1
     const int wk = warp & (along_k - 1), wr = warp >> p.along_shift;
@@ -480,8 +543,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     if (lane == 0)
         for (int i = 0; i < p.depth; ++i)
             mbar_init(&full[i], 1);
-    if (threadIdx.x < 18)
-        largest[threadIdx.x] = 0;
+    if (threadIdx.x < 16) {
+        notes.largest[threadIdx.x] = 0;
+        notes.exponent[threadIdx.x] = ROW_EXPONENT;
+    }
+    if (threadIdx.x == 0)
+        notes.lossy = notes.odd = 0;
     fence_barrier_init();
     fence_proxy_async();
     __syncthreads();
@@ -496,168 +563,155 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     const int token_turn = warp / tokens, token = warp - token_turn * tokens;
     const int first_piece = token_turn < token_warps ? token_turn * 32 + lane : token_pieces, step = token_warps * 32;
     const T* x_row = static_cast<const T*>(p.x) + (token0 + token) * p.x_stride;
-    auto put = [&](int of, int i, const T (&raw)[8], float up_by) {
-        float pairs[4][2];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            pairs[j / 2][j % 2] = to_f32(raw[j]) * up_by;
-        uint8_t* dst = xs + of * 64 + (i >> 2) * p.tokens * 64 + (i & 3) * 16;
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part)
-            *reinterpret_cast<uint4*>(dst + part * x_plane)
-                = make_uint4(take_half_pair(pairs[0]), take_half_pair(pairs[1]), take_half_pair(pairs[2]), take_half_pair(pairs[3]));
-    };
-    // 32-bit rows are looked at first.  bfloat16 rows are multiplied by 2^6 at once, and only those with a number that this does not suit
-    // (two at a time, their bits as whole numbers; less 1, so that a zero is the largest of all) are looked at, and done once more by
-    // the whole CTA: 8 rows through a gated pair of 2 x 12,288 x 4,096 16.7 us, with one such row 17.8, all of them such 21.9.
     constexpr float AT_FIRST = float(1 << ROW_EXPONENT);
-    uint32_t most_two = 0, least_two = 0xffffffffu;
-    auto put_at_first = [&](int i, const T (&raw)[8]) {
-        put(token, i, raw, AT_FIRST);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t two = reinterpret_cast<const uint32_t*>(raw)[j] & 0x7fff7fffu;
-            most_two = __vmaxu2(most_two, two);
-            least_two = __viaddmin_u16x2(two, 0xffffffffu, least_two);
-        }
-    };
-    float most_of = 0.f;
-    auto look = [&](const T (&raw)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            most_of = fmaxf(most_of, fabsf(to_f32(raw[j])));
-    };
-    auto look_at_finite = [&](const T (&raw)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            most_of = fabsf(to_f32(raw[j])) < INFINITY ? fmaxf(most_of, fabsf(to_f32(raw[j]))) : most_of;
-    };
-    // pieces of a row whose largest number is known, with its factor, and whether they have numbers that lose bits
-    auto put_and_note = [&](int of, const T* row, int piece0, int pieces) {
-        const int e = row_exponent(largest[of]);
-        uint32_t smallest = 0xffffffffu;         // but zero, its bits less 1
+    auto put = [&](int i, const T (&raw)[8], float up_by) { put_piece(xs + token * 64 + (i >> 2) * p.tokens * 64 + (i & 3) * 16, x_plane, raw, up_by); };
+    // A row's factor wants its largest number before any is converted.  32-bit rows are fetched twice, unless a thread's pieces fit its
+    // registers and wait there.  bfloat16 rows are multiplied by 2^6 at once, and only those with a number that this does not suit (two at
+    // a time, their bits as whole numbers; less 1, so that a zero is the largest of all) once more (put_rows_again):
+    // one row of 4,096 x 4,096 4.8 us, such a one 6.2; 8 rows through a gated pair of 2 x 12,288 x 4,096 16.9, with one such 18.4.
+    const bool whole = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)p.x_stride * sizeof(T)) & 15) == 0 && (p.k & 7) == 0;  // on 16 bytes
+    const int there = min(token_pieces, (p.k - c0 * PACKED_COLS) >> 3);
+    const T* src = x_row + c0 * PACKED_COLS;
+    // calls f for this thread's pieces: AT_ONCE on their way, one copy of f's code (what a kernel runs once it waits for)
+    auto each_piece = [&](auto f) {
+        constexpr int AT_ONCE = X32 ? 2 : 4;
+        if (whole) {
 #pragma unroll 1
-        for (int i = piece0; i < token_pieces; i += pieces) {
-            __align__(16) T raw[8];
-            read_eight(row, (c0 * 16 + i) * 8, p.k, raw);
-            put(of, i, raw, power_of_two(e));
+            for (int i0 = first_piece; i0 < token_pieces; i0 += AT_ONCE * step) {
+                __align__(16) T raw[AT_ONCE][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                smallest = __viaddmin_u32(__float_as_uint(to_f32(raw[j])) & 0x7fffffffu, 0xffffffffu, smallest);
-        }
-        if (smallest < __float_as_uint(least_kept<X32>() * power_of_two(-e)) - 1)
-            atomicOr(&largest[16], 1u << of);
-    };
-    if (((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)p.x_stride * sizeof(T)) & 15) == 0 && (p.k & 7) == 0) {
-        // whole pieces on 16 bytes
-        constexpr int AT_ONCE = X32 ? 2 : 4;     // pieces of a thread on their way
-        const int there = min(token_pieces, (p.k - c0 * PACKED_COLS) >> 3);
-        const T* src = x_row + c0 * PACKED_COLS;
+                for (int a = 0; a < AT_ONCE; ++a)
+#pragma unroll
+                    for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+                        reinterpret_cast<uint4*>(raw[a])[h]
+                            = i0 + a * step < there ? reinterpret_cast<const uint4*>(src + (i0 + a * step) * 8)[h] : make_uint4(0, 0, 0, 0);
 #pragma unroll 1
-        for (int i0 = first_piece; i0 < token_pieces; i0 += AT_ONCE * step) {
-            __align__(16) T raw[AT_ONCE][8];
+                for (int i = i0; i < min(i0 + AT_ONCE * step, token_pieces); i += step) {
+                    f(i, raw[0]);
 #pragma unroll
-            for (int a = 0; a < AT_ONCE; ++a)
+                    for (int a = 0; a + 1 < AT_ONCE; ++a)
 #pragma unroll
-                for (int h = 0; h < (int)sizeof(T) / 2; ++h)
-                    reinterpret_cast<uint4*>(raw[a])[h]
-                        = i0 + a * step < there ? reinterpret_cast<const uint4*>(src + (i0 + a * step) * 8)[h] : make_uint4(0, 0, 0, 0);
-            // (one copy of the code for all of them: what a kernel runs once it waits for)
-#pragma unroll 1
-            for (int i = i0; i < min(i0 + AT_ONCE * step, token_pieces); i += step) {
-                if constexpr (X32)
-                    look(raw[0]);
-                else
-                    put_at_first(i, raw[0]);
-#pragma unroll
-                for (int a = 0; a + 1 < AT_ONCE; ++a)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        raw[a][j] = raw[a + 1][j];
+                        for (int j = 0; j < 8; ++j)
+                            raw[a][j] = raw[a + 1][j];
+                }
             }
-        }
-    } else {
-#pragma unroll 1
-        for (int i = first_piece; i < token_pieces; i += step) {
-            __align__(16) T raw[8];
-            read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
-            if constexpr (X32)
-                look(raw);
-            else
-                put_at_first(i, raw);
-        }
-    }
-    uint32_t own_factor = 0;                     // the rows with a factor of their own
-    if constexpr (X32) {
-        uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
-        if (warps_most == 0x7f800000u) {         // (an infinity: the largest of the others; fmaxf passes NaN over)
-            most_of = 0.f;
+        } else {
 #pragma unroll 1
             for (int i = first_piece; i < token_pieces; i += step) {
                 __align__(16) T raw[8];
                 read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
-                look_at_finite(raw);
+                f(i, raw);
             }
-            warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
         }
-        if (lane == 0)
-            atomicMax(&largest[token], warps_most);
+    };
+    if constexpr (X32) {
+        // the largest finite magnitude among this warp's pieces (`most`: the largest of all) into its row's
+        auto note_most = [&](float of_all) {
+            uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(of_all));
+            if (most == 0x7f800000u) {           // (an infinity aside)
+                float finite = 0.f;
+#pragma unroll 1
+                for (int i = first_piece; i < token_pieces; i += step) {
+                    __align__(16) T raw[8];
+                    read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        finite = fabsf(raw[j]) < INFINITY ? fmaxf(finite, fabsf(raw[j])) : finite;
+                }
+                most = __reduce_max_sync(0xffffffffu, __float_as_uint(finite));
+            }
+            if (lane == 0)
+                atomicMax(&notes.largest[token], most);
+        };
+        uint32_t smallest = 0xffffffffu;         // but zero, its bits less 1
+        auto note_row = [&](int e) {
+            if (smallest < __float_as_uint(least_kept<X32>() * power_of_two(-e)) - 1)
+                atomicOr(&notes.lossy, 1u << token);
+            if (lane == 0)
+                notes.exponent[token] = e;
+        };
+        auto put_and_note = [&](int i, const T (&raw)[8], int e) {
+            put(i, raw, power_of_two(e));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                smallest = __viaddmin_u32(__float_as_uint(raw[j]) & 0x7fffffffu, 0xffffffffu, smallest);
+        };
+        float most = 0.f;                        // (fmaxf passes NaN over)
+        auto look = [&](const T (&raw)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                most = fmaxf(most, fabsf(raw[j]));
+        };
+        constexpr int KEPT = 4;
+        if (whole && token_pieces <= KEPT * step) {
+            __align__(16) T raw[KEPT][8];
+#pragma unroll
+            for (int a = 0; a < KEPT; ++a)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    reinterpret_cast<uint4*>(raw[a])[h] = first_piece + a * step < there
+                        ? reinterpret_cast<const uint4*>(src + (first_piece + a * step) * 8)[h] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int a = 0; a < KEPT; ++a)
+                look(raw[a]);
+            note_most(most);
+            __syncthreads();
+            const int e = row_exponent(notes.largest[token]);
+#pragma unroll 1
+            for (int i = first_piece; i < token_pieces; i += step) {
+                put_and_note(i, raw[0], e);
+#pragma unroll
+                for (int a = 0; a + 1 < KEPT; ++a)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        raw[a][j] = raw[a + 1][j];
+            }
+            note_row(e);
+        } else {
+            each_piece([&](int, const T (&raw)[8]) { look(raw); });
+            note_most(most);
+            __syncthreads();
+            const int e = row_exponent(notes.largest[token]);
+#pragma unroll 1
+            for (int i = first_piece; i < token_pieces; i += step) {
+                __align__(16) T raw[8];
+                read_eight(x_row, (c0 * 16 + i) * 8, p.k, raw);
+                put_and_note(i, raw, e);
+            }
+            note_row(e);
+        }
         __syncthreads();
-        put_and_note(token, x_row, first_piece, step);
-        __syncthreads();
-        own_factor = 0xffffffffu;
     } else {
+        uint32_t most_two = 0, least_two = 0xffffffffu;
+        each_piece([&](int i, const T (&raw)[8]) {
+            put(i, raw, float(1 << ROW_EXPONENT));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t two = reinterpret_cast<const uint32_t*>(raw)[j] & 0x7fff7fffu;
+                most_two = __vmaxu2(most_two, two);
+                least_two = __viaddmin_u16x2(two, 0xffffffffu, least_two);
+            }
+        });
         const bool odd = max(most_two >> 16, most_two & 0xffffu) >= ROW_MOST << 7 || min(least_two >> 16, least_two & 0xffffu) < (ROW_LEAST << 7) - 1;
         if (odd)
-            atomicOr(&largest[17], 1u << token);
-        if (__builtin_expect(__syncthreads_or(odd), false)) {
-            own_factor = largest[17];
-            // (the warps share them as they shared all)
-            const int rows = __popc(own_factor), turn = warp / rows, each = p.warps / rows;
-            uint32_t from = own_factor;
-            for (int skip = warp - turn * rows; skip > 0; --skip)
-                from &= from - 1;
-            const int of = __ffs(from) - 1;
-            const int piece0 = turn < each ? turn * 32 + lane : token_pieces;
-            const T* row = x_row + (of - token) * p.x_stride;
-#pragma unroll 1
-            for (int i = piece0; i < token_pieces; i += each * 32) {
-                __align__(16) T raw[8];
-                read_eight(row, (c0 * 16 + i) * 8, p.k, raw);
-                look_at_finite(raw);
-            }
-            const uint32_t warps_most = __reduce_max_sync(0xffffffffu, __float_as_uint(most_of));
-            if (lane == 0)
-                atomicMax(&largest[of], warps_most);
-            __syncthreads();
-            put_and_note(of, row, piece0, each * 32);
-            __syncthreads();
-        }
+            atomicOr(&notes.odd, 1u << token);
+        if (__builtin_expect(__syncthreads_or(odd), false))
+            put_rows_again(p, xs, notes, token0, c0, token_pieces);
     }
 
     // ---- the stream
     const int r = lane >> 2, c = lane & 3;
     const uint32_t code_at = (uint32_t)packed_word_at(r, c);
     uint32_t x_lane[NT];
-    float down[NT][2];                           // undo the rows' factors
+    float down[NT][2];                           // undo the rows' factors and the codes'
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         x_lane[t] = (uint32_t)min(t * 8 + r, tokens - 1) * 64 + c * 16;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            down[t][j] = 1.f / AT_FIRST;
+            down[t][j] = power_of_two(PACKED_HALF_EXPONENT - notes.exponent[min(t * 8 + 2 * c + j, tokens - 1)]);
     }
-    uint32_t lossy = 0;                          // the rows with numbers that lost bits
-    if (__builtin_expect(own_factor != 0, X32)) {
-        lossy = largest[16];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int of = min(t * 8 + 2 * c + j, tokens - 1);
-                down[t][j] = own_factor >> of & 1 ? power_of_two(-row_exponent(largest[of])) : down[t][j];
-            }
-    }
+    const uint32_t lossy = notes.lossy;
     const uint32_t x_block = (uint32_t)p.tokens * 64;
     bool dead = false;                           // a wait ran out: nothing more is asked for
     int slot = 0;
@@ -756,7 +810,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
             __syncwarp();
             for (int u = 0; u < min(now, warp_rounds - first); ++u)
                 add_what_was_lost<X32, NT>(p, lossy, token0, (cluster + (first + u) * p.clusters) * blocks_per_unit + wr, w0, w1,
-                                           GROUP_BLOCKS * 32, largest, sums + (u * p.warps + warp) * SUMS);
+                                           GROUP_BLOCKS * 32, notes, sums + (u * p.warps + warp) * SUMS);
         }
 
         // ---- the cluster adds up what its warps have
@@ -776,13 +830,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
         }
         const int rows_out = p.pair ? PACKED_ROWS / 2 : PACKED_ROWS;
         const int outputs = now * blocks_per_unit * rows_out * tokens;
-        for (int e0 = rank * blockDim.x + warp * 32; e0 < outputs; e0 += splits * blockDim.x) {
-            const int e = min(e0 + lane, outputs - 1);
+        for (int e = rank * blockDim.x + threadIdx.x; e < outputs; e += splits * blockDim.x) {
             const int row = e & (rows_out - 1), rest = e >> (p.pair ? 4 : 5);
             const int block = rest / tokens, token = rest - block * tokens;          // block: of the batch, unit by unit
             const int u = block >> unit_shift, b = block & (blocks_per_unit - 1);
-            const int block_at = (cluster + (first + u) * p.clusters) * blocks_per_unit + b, at = block_at * rows_out + row;
-            const bool there = e0 + lane < outputs && at < p.n;
+            const int at = ((cluster + (first + u) * p.clusters) * blocks_per_unit + b) * rows_out + row;
+            if (at >= p.n)
+                continue;
             // the fragment's place of (row of the record, token); a pair's up lies two registers behind its gate
             const int in_record = p.pair ? (row >> 3) * 16 + (row & 7) : row;
             const int reg = ((in_record >> 4) * NT + (token >> 3)) * 4 + ((in_record >> 3) & 1) * 2 + (token & 1);
@@ -803,14 +857,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
                         up += place[w * SUMS + 64];
                 }
             }
-            // (sums that passed 2^128, or x or a scale that is no number)
-            if (__builtin_expect(__any_sync(0xffffffffu, there && !(fabsf(v) + fabsf(up) < INFINITY)), false)) {
-                const float2 both = sums_in_64_bits<X32>(p, GROUP_BLOCKS * 32, there, block_at, in_record, token0 + token, make_float2(v, up));
-                v = both.x;
-                up = both.y;
-            }
-            if (!there)
-                continue;
             if (p.pair)
                 v = (p.out_type == CHIBI_F32 ? packed_activate<false>(v, p.act) : packed_activate<true>(v, p.act)) * up;
             const long long m = token0 + token;
@@ -842,7 +888,7 @@ size_t few_rows_smem(bool x32, int group, int chunks, int warps, int splits, int
 {
     const size_t x_plane = (size_t)((chunks + splits - 1) / splits) * 4 * tokens * 64;
     return (size_t)warps * depth * ((run * packed_record_bytes(group) + 127) / 128 * 128) + (x32 ? 2 : 1) * x_plane
-        + (size_t)batch * warps * 256 * (tokens <= 8 ? 1 : 2) * 4 + 18 * 4 + warps * depth * 8;
+        + (size_t)batch * warps * 256 * (tokens <= 8 ? 1 : 2) * 4 + sizeof(RowNotes) + warps * depth * 8;
 }
 
 void (*few_rows_kernel(bool x32, int tokens, int group))(const CUtensorMap, const FewRows)

@@ -191,9 +191,10 @@ class CudaKernels:
         self._attention_tc_libs = {}
         self._attention_tied_libs = {}
         self.use_tcgen05_attention = True
-        # matrices in 4 bits: up to so many bfloat16 rows of x stream the matrix once through mma.sync, more go to tcgen05 (12 rows of
-        # 4,096 x 4,096 8.6 against 9.9 us, of 151,936 x 4,096 117 against 145, of a gated pair of 2 x 12,288 x 4,096 24.6 against 30.1; 16 rows
-        # 8.9 against 10.0, 132 against 145, 33 against 30; tcgen05's times hardly change up to 48 rows)
+        # matrices in 4 bits: up to so many bfloat16 rows of x stream the matrix once through mma.sync, more go to tcgen05, whose times
+        # hardly change up to 48 rows.  (12 rows of 4,096 x 4,096 8.7 against 9.9 us, of 151,936 x 4,096 119 against 143, of a gated pair of
+        # 2 x 12,288 x 4,096 24.5 against 29.6; 16 rows 8.8 against 9.9, 133 against 143, but 6,144 x 4,096 15.0 against 12.9 and the pair
+        # 33.3 against 29.7: one number for all shapes gives 10 to 16 % away there.  20 rows 10.7 against 10.0, 185 against 143.)
         self.packed_few_rows_max = 16
         # (by sizes, for all kernels of a process on this device)
         self._packed_plans: Dict[tuple, FewRowsPlan] = _PACKED_PLANS.setdefault(self._device_index, {})
@@ -736,7 +737,8 @@ class CudaKernels:
         in flight on the stream writes it (32-bit products wait first).
         With ``defer`` (together with a residual that aliases out, or without one) a split
         product is left pending -- the caller adds it, or takes it for ``out`` -- and is returned.
-        ``w`` may be PackedWeights (not a pair): any x and out of the two types."""
+        ``w`` may be PackedWeights (not a pair): any x and out of the two types.  (Sums are in 32 bits on the way: weights from
+        10^36 on may make a finite product infinite.)"""
         if isinstance(w, PackedWeights):
             return self._packed_product(x, w, out, residual, None, "linear")
         if isinstance(x, ScaledRows):
