@@ -24,7 +24,9 @@ class LLM:
 
     ``weight_group`` (32, 64 or 128) puts the matrices of attention, of dense feed-forwards and of the output into 4 bits
     while the model is loaded, with a bfloat16 scale for so many neighbouring columns of a row
-    (the reference's load-time ``--quantize q4``; here symmetric, without offsets)."""
+    (the reference's load-time ``--quantize q4``; here symmetric, without offsets).  Steps of few requests take about half
+    as long; prompts from a few hundred tokens on up to 1.5 times as long as with bfloat16 matrices.  Experts,
+    recurrences and latent attention stay as they are."""
 
     def __init__(self, model_dir: Optional[str], dtype: str = "bfloat16", device: str = "cuda:0",
                  context_length: int = 4096, kv_cache_tokens: Optional[int] = None,

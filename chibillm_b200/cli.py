@@ -38,7 +38,8 @@ USAGE = """Usage: python -m chibillm_b200 [--context-length N] [--max-tokens N] 
   --context-length N  Prompt + output capacity (default: 32768; multiple of the page size)
   --max-tokens N      Reply limit (default: 8192)
   --quantize none     Only 'none': the reference's affine 4-bit weights are not built in this engine
-  --weight-group G    Matrices in 4 bits with a scale for every G columns of a row (32, 64 or 128)
+  --weight-group G    Matrices in 4 bits with a scale for every G columns of a row (32, 64 or 128):
+                      faster decoding of few requests, slower long prompts; experts stay as they are
   --prompt-cache-mib 0  Only 0: the prefix cache is not built in this engine
   --no-stream         Print replies only when complete
   --progress=auto|off  Prefill progress on terminals (default: auto)

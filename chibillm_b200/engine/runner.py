@@ -124,7 +124,8 @@ class ModelRunner:
                     pool_tokens: int = 4096, max_requests: int = 4, kernels=None,
                     weight_group: Optional[int] = None) -> "ModelRunner":
         """``weight_group``: None keeps the matrices as the checkpoint has them; 32, 64 or 128 puts those of attention and dense
-        feed-forwards and the output matrix into 4 bits while they are bound, with a scale for so many columns of a row."""
+        feed-forwards and the output matrix into 4 bits while they are bound, with a scale for so many columns of a row
+        (experts, recurrences and latent attention stay)."""
         _, _, spec = load_config(model_dir)
         runtime = make_runtime(dtype, device, kernels, spec, weight_group)
         model = DecoderModel(spec, runtime)
