@@ -94,7 +94,7 @@ inline bool packed_map(const void* data, int group, int row_blocks, int col_bloc
 // The whole numbers of a word as float16, columns 2 j and 2 j + 1 in pair j, times 2^-14 (exact: 1,024 + code and 1,024 + 16 code have
 // the code in float16's ten bits of mantissa, a way that open 4-bit kernels share; what is taken off leaves a small whole number).
 // x is held at 2^15 at most, so a group's sum is below 2^11 and its product with a scale finite for scales below 2^117, weights of
-// 10^36.  PACKED_HALF_EXPONENT undoes it.
+// 10^36; for weights below 10^-35 it comes into the range where 32-bit numbers have fewer bits.  PACKED_HALF_EXPONENT undoes it.
 constexpr int PACKED_HALF_EXPONENT = 14;
 __device__ __forceinline__ void packed_half_pairs(uint32_t word, uint32_t (&pair)[4])
 {

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // numbers from 2^-9 on.  What is smaller (bfloat16: 2^-14, 32-bit: 2^-9, as multiplied) and lost bits is added to the warps' sums in
 // 32 bits after the stream, so nothing vanishes beside a large number whose weights are zeros (add_what_was_lost; a row of 4,096 normal
 // numbers has one with a chance of 1e-5, a 32-bit one of 1e-3; one such number makes the product with 4,096 x 4,096 take 7.4 us
-// instead of 4.8, a row of nothing else 36).
+// instead of 4.8, a row of nothing else 31).
 //
 // How the work is shared out (CudaKernels.packed_plan chooses): `splits` CTAs of a cluster share the columns, `along_k`
 // warps of a CTA share the CTA's columns of one block of 32 rows, the CTA's warps / along_k blocks of rows are a unit, and clusters
@@ -446,8 +446,8 @@ template <typename T> __device__ __forceinline__ void put_piece(uint8_t* to, uin
             = make_uint4(take_half_pair(pairs[0]), take_half_pair(pairs[1]), take_half_pair(pairs[2]), take_half_pair(pairs[3]));
 }
 
-// bfloat16 rows that the first factor does not suit, once more, by all warps; `piece`s of a row's columns c0 * 128 ....  Begins
-// and ends with the CTA together.
+// bfloat16 rows that the first factor does not suit, once more, by all warps: `pieces` of 8 columns from block c0 on.  Begins and ends
+// with the CTA together.
 __device__ __noinline__ void put_rows_again(const FewRows& p, uint8_t* xs, RowNotes& notes, int token0, int c0, int pieces)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     } else {
         uint32_t most_two = 0, least_two = 0xffffffffu;
         each_piece([&](int i, const T (&raw)[8]) {
-            put(i, raw, float(1 << ROW_EXPONENT));
+            put(i, raw, AT_FIRST);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t two = reinterpret_cast<const uint32_t*>(raw)[j] & 0x7fff7fffu;

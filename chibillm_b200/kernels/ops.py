@@ -738,7 +738,7 @@ class CudaKernels:
         With ``defer`` (together with a residual that aliases out, or without one) a split
         product is left pending -- the caller adds it, or takes it for ``out`` -- and is returned.
         ``w`` may be PackedWeights (not a pair): any x and out of the two types.  (Sums are in 32 bits on the way: weights from
-        10^36 on may make a finite product infinite.)"""
+        10^36 on may make a finite product infinite, below 10^-35 cost it last bits.)"""
         if isinstance(w, PackedWeights):
             return self._packed_product(x, w, out, residual, None, "linear")
         if isinstance(x, ScaledRows):

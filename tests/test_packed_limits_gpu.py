@@ -251,3 +251,18 @@ def test_a_residual_beside_bfloat16_outputs(kernels, m, x_dtype):
     bound = off_by(x, values, 64, F32, want) + want.abs() * 2.0 ** -24
     want = want + add.double()
     close(out, want, bound * (1 + 2.0 ** -8) + want.abs() * 2.0 ** -8)
+
+
+@pytest.mark.parametrize("m", [1, 16, 17, 200])
+@pytest.mark.parametrize("scale", [2.0 ** -113, 2.0 ** -100, 2.0 ** 100, 2.0 ** 116])
+def test_weights_of_every_size(kernels, m, scale):
+    """Scales from 2^-113 to 2^116 (weights of 10^-33 to 10^36) with x of about one, and with x that brings the product back to one."""
+    g = gen(73 + m)
+    codes, _, x = whole_numbers(g, m, 70, 600, 64, BF16)
+    scales = torch.full((70, 10), scale, dtype=BF16, device=DEV)
+    packed, values = kernels.pack_codes(codes, scales, 64), values_of(codes, scales, 64)
+    out = torch.empty(m, 70, device=DEV)
+    for rows in (x if scale < 1 else x * 2.0 ** -10, (x.float() / scale).to(BF16)):
+        kernels.linear(rows, packed, out)
+        # (600 * 8 * 15 < 2^17 steps of the product's own size: exact, its smallest step above 2^-149)
+        assert torch.equal(out.double(), rows.double() @ values.t())
