@@ -91,22 +91,22 @@ inline bool packed_map(const void* data, int group, int row_blocks, int col_bloc
               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The whole numbers of a word as float16, columns 2 j and 2 j + 1 in pair j, times 2^-14 (exact: 1,024 + code and 1,024 + 16 code have
-// the code in float16's ten bits of mantissa, a way that open 4-bit kernels share; what is taken off leaves a small whole number).
+// The whole numbers of a word as float16, columns 2 j and 2 j + 1 in pair j, times 2^-14 (exact: 2^-4 + 2^-14 code and 2^-4 + 2^-10 code
+// have the code in float16's ten bits of mantissa, a way that open 4-bit kernels share; what is taken off leaves a small number).
 // x is held at 2^15 at most, so a group's sum is below 2^11 and its product with a scale finite for scales below 2^117, weights of
 // 10^36; for weights below 10^-35 it comes into the range where 32-bit numbers have fewer bits.  PACKED_HALF_EXPONENT undoes it.
 constexpr int PACKED_HALF_EXPONENT = 14;
 __device__ __forceinline__ void packed_half_pairs(uint32_t word, uint32_t (&pair)[4])
 {
     const uint32_t next = word >> 8;
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(pair[0]) : "r"(word));
-    asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(pair[1]) : "r"(word));
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(pair[2]) : "r"(next));
-    asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(pair[3]) : "r"(next));
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[0]) : "r"(0x04000400u), "r"(0xac08ac08u)); // * 2^-14 - 1,032 * 2^-14
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[1]) : "r"(0x00400040u), "r"(0x9c809c80u)); // * 2^-18 - 1,152 * 2^-18
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[2]) : "r"(0x04000400u), "r"(0xac08ac08u));
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[3]) : "r"(0x00400040u), "r"(0x9c809c80u));
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x2c002c00, 0xea;" : "=r"(pair[0]) : "r"(word));
+    asm("lop3.b32 %0, %1, 0x00f000f0, 0x2c002c00, 0xea;" : "=r"(pair[1]) : "r"(word));
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x2c002c00, 0xea;" : "=r"(pair[2]) : "r"(next));
+    asm("lop3.b32 %0, %1, 0x00f000f0, 0x2c002c00, 0xea;" : "=r"(pair[3]) : "r"(next));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(pair[0]) : "r"(0x2c082c08u));                       // - 1,032 * 2^-14
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[1]) : "r"(0x2c002c00u), "r"(0x9c809c80u)); // / 16 - 72 * 2^-14
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(pair[2]) : "r"(0x2c082c08u));
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(pair[3]) : "r"(0x2c002c00u), "r"(0x9c809c80u));
 }
 
 // The same as bfloat16, times 2^-10 (2^-3 + 2^-10 code has its code in the lowest of bfloat16's seven bits of mantissa).  A group's

@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(512, 4) unpack_kernel(const uint8_t* __restric
 // (each CTA its warps, then CTA by CTA), each CTA a share of the outputs, so the same plan gives the same bits.
 //
 // Measured (replayed in a graph, matrices out of L2): one row of 2,048 x 1,024 3.0 us, of 4,096 x 4,096 4.8, of 4,096 x 12,288 9.0, of a gated
-// pair of 2 x 12,288 x 4,096 13.3 (4.0 TB/s); four rows of 151,936 x 4,096 65.2 (5.1 TB/s), 284 instructions a record at 2.55 a
-// cycle and SM; 12 32-bit rows of a pair of 2 x 2,730 x 1,024 6.4.  Before and after the stream of one row go by 2.5 us: a kernel's start, x from
+// pair of 2 x 12,288 x 4,096 13.2 (4.1 TB/s); four rows of 151,936 x 4,096 64.6 (5.1 TB/s), 284 instructions a record at 2.55 a
+// cycle and SM; 12 32-bit rows of a pair of 2 x 2,730 x 1,024 6.3.  Before and after the stream of one row go by 2.5 us: a kernel's start, x from
 // L2, a barrier, the warps' sums.
 constexpr int FEW_THREADS = 512;             // at most
 
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) packed_few_rows_kernel(const _
     // A row's factor wants its largest number before any is converted.  32-bit rows are fetched twice, unless a thread's pieces fit its
     // registers and wait there.  bfloat16 rows are multiplied by 2^6 at once, and only those with a number that this does not suit (two at
     // a time, their bits as whole numbers; less 1, so that a zero is the largest of all) once more (put_rows_again):
-    // one row of 4,096 x 4,096 4.8 us, such a one 6.2; 8 rows through a gated pair of 2 x 12,288 x 4,096 16.9, with one such 18.4.
+    // one row of 4,096 x 4,096 4.8 us, such a one 6.2; 8 rows through a gated pair of 2 x 12,288 x 4,096 16.8, with one such 18.3.
     const bool whole = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)p.x_stride * sizeof(T)) & 15) == 0 && (p.k & 7) == 0;  // on 16 bytes
     const int there = min(token_pieces, (p.k - c0 * PACKED_COLS) >> 3);
     const T* src = x_row + c0 * PACKED_COLS;

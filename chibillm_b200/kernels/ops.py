@@ -193,8 +193,8 @@ class CudaKernels:
         self.use_tcgen05_attention = True
         # matrices in 4 bits: up to so many bfloat16 rows of x stream the matrix once through mma.sync, more go to tcgen05, whose times
         # hardly change up to 48 rows.  (12 rows of 4,096 x 4,096 8.7 against 9.9 us, of 151,936 x 4,096 119 against 143, of a gated pair of
-        # 2 x 12,288 x 4,096 24.5 against 29.6; 16 rows 8.8 against 9.9, 133 against 143, but 6,144 x 4,096 15.0 against 12.9 and the pair
-        # 33.3 against 29.7: one number for all shapes gives 10 to 16 % away there.  20 rows 10.7 against 10.0, 185 against 143.)
+        # 2 x 12,288 x 4,096 24.8 against 29.6; 16 rows 8.8 against 9.9, 133 against 143, but 6,144 x 4,096 15.1 against 12.9 and the pair
+        # 33.6 against 29.7: one number for all shapes gives 10 to 16 % away there.  20 rows 10.7 against 10.0, 185 against 143.)
         self.packed_few_rows_max = 16
         # (by sizes, for all kernels of a process on this device)
         self._packed_plans: Dict[tuple, FewRowsPlan] = _PACKED_PLANS.setdefault(self._device_index, {})
